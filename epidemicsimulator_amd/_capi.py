@@ -80,6 +80,12 @@ class WorldDesc(C.Structure):
                 ("hp", CHyper), ("device", C.c_int32), ("pad_", C.c_int32)]
 
 
+class LayerDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int64), ("x_stride", C.c_int64), ("y_stride", C.c_int64),
+                ("dy_stride", C.c_int64), ("eps", C.c_double), ("dropout", C.c_double), ("seed", C.c_int64),
+                ("offset", C.c_int64), ("offset_dev", C.c_void_p), ("dtype", C.c_int32), ("device", C.c_int32)]
+
+
 # Every symbol include/epi.h declares; tests check that the library exports all of them.
 EXPORTED_SYMBOLS = [
     "epi_version", "epi_last_error", "epi_last_status", "epi_device_count", "epi_set_device", "epi_alloc_int", "epi_alloc_int_batch",
@@ -93,6 +99,7 @@ EXPORTED_SYMBOLS = [
     "epi_agents_create", "epi_agents_destroy", "epi_agents_observe", "epi_agents_observe_world", "epi_agents_replay_size", "epi_agents_sample",
     "epi_agents_learn", "epi_agents_q_values", "epi_agents_get_weights", "epi_agents_set_weights",
     "epi_agents_set_timing", "epi_agents_kernel_time",
+    "epi_dropout", "epi_layer_norm_forward", "epi_layer_norm_backward_workspace", "epi_layer_norm_backward",
 ]
 
 _lib = None
@@ -162,6 +169,11 @@ def lib():
         L.epi_agents_set_weights.argtypes = [C.c_void_p, C.c_int32, C.c_int32] + [_PD] * 6
         L.epi_agents_set_timing.argtypes = [C.c_void_p, C.c_int32]
         L.epi_agents_kernel_time.argtypes = [C.c_void_p, C.POINTER(C.c_double), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]
+        layer = C.POINTER(LayerDesc)
+        L.epi_dropout.argtypes = [layer] + [C.c_void_p] * 3
+        L.epi_layer_norm_forward.argtypes = [layer] + [C.c_void_p] * 7
+        L.epi_layer_norm_backward_workspace.argtypes = [layer, C.POINTER(C.c_size_t)]
+        L.epi_layer_norm_backward.argtypes = [layer] + [C.c_void_p] * 9 + [C.c_size_t, C.c_void_p]
         for name in ("epi_world_destroy", "epi_world_reset"):
             getattr(L, name).argtypes = [C.c_void_p]
         _lib = L

@@ -1,0 +1,702 @@
+// Layer operators on device memory: dropout whose mask is computed from a counter and never stored, layer
+// normalisation with its backward pass, and both in one pass, y = norm(dropout(x)).
+//
+//   dropout   d(x) = x * 65536 / (65536 - t) where the unit's 16-bit draw is >= t, else 0; its gradient is d(dy)
+//   norm      h = x or d(x);  m = mean h;  r = 1 / sqrt(mean (h - m)^2 + eps);  u = (h - m) r;  y = u w + b
+//   backward  g = dy w;  dh = r (g - mean g - u mean(g u));  dx = dh or d(dh);  dw = sum dy u;  db = sum dy
+//
+// Sums, means and the values between load and store are floats for float, bfloat16 and half, doubles for double; a
+// value is rounded to its type once, as it is stored.  All of it is bound by memory: a thread takes chunks of eight
+// consecutive columns (one counter of the generator, 16 bytes of a 16-bit type), and the work between is hidden
+// behind the loads -- ten rounds of the generator for every chunk of a dropout of 819,200 x 128 bfloat16 leave it at
+// the rate of a copy (69.9 us, 6.0 TB/s, with them and 70.4 us without).
+#include "epi_layers.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "epi_host.hpp"
+
+#define EPI_API extern "C" __attribute__((visibility("default")))
+
+namespace epi {
+namespace {
+
+constexpr int kChunk = 8;   // columns a thread takes at once: the eight draws of one counter
+
+template <class T> struct Wide { using type = float; };
+template <> struct Wide<double> { using type = double; };
+template <class T> using wide_t = typename Wide<T>::type;
+
+// ---- chunks of eight columns ------------------------------------------------------------------
+// Rows of odd widths start at any multiple of the element's size, so the vectors are declared with the element's
+// alignment: the hardware takes 16-byte accesses at any address, and rows that do start at 16 bytes lose nothing.
+template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Chunk { T v[kChunk]; };
+
+template <class T>
+__device__ inline void load_chunk(const T* p, int count, wide_t<T> (&out)[kChunk]) {
+    if (count >= kChunk) {
+        const Chunk<T> c = *reinterpret_cast<const Chunk<T>*>(p);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) out[k] = (wide_t<T>)c.v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) out[k] = k < count ? (wide_t<T>)p[k] : (wide_t<T>)0;
+    }
+}
+
+template <class T>
+__device__ inline void store_chunk(T* p, int count, const wide_t<T> (&in)[kChunk]) {
+    if (count >= kChunk) {
+        Chunk<T> c;
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) c.v[k] = (T)in[k];
+        *reinterpret_cast<Chunk<T>*>(p) = c;
+    } else {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k)
+            if (k < count) p[k] = (T)in[k];
+    }
+}
+
+// ---- the generator ------------------------------------------------------------------------------
+// The four words of Philox4x32-10 for chunk `chunk` of row `row`.
+__device__ inline void draw_words(const DropArgs& d, const uint32_t (&off)[2], uint32_t chunk, uint32_t row, uint32_t (&w)[4]) {
+    uint32_t c0 = chunk, c1 = row, c2 = off[0], c3 = off[1], k0 = d.key[0], k1 = d.key[1];
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+        const uint64_t p = (uint64_t)0xD2511F53u * c0, q = (uint64_t)0xCD9E8D57u * c2;
+        c0 = (uint32_t)(q >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)q;
+        c2 = (uint32_t)(p >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)p;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    w[0] = c0; w[1] = c1; w[2] = c2; w[3] = c3;
+}
+
+__device__ inline void drop_offset(const DropArgs& d, uint32_t (&off)[2]) {
+    uint64_t o = ((uint64_t)d.offset[1] << 32) | d.offset[0];
+    if (d.offset_dev) o += (uint64_t)*d.offset_dev;
+    off[0] = (uint32_t)o; off[1] = (uint32_t)(o >> 32);
+}
+
+// A dropped value becomes zero whatever it was: infinities and NaN do not pass through the product.
+template <class A>
+__device__ inline void drop_chunk(const DropArgs& d, A scale, const uint32_t (&w)[4], A (&v)[kChunk]) {
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+        const uint32_t draw = (k & 1) ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu;
+        v[k] = draw >= d.threshold ? v[k] * scale : (A)0;
+    }
+}
+
+// ---- sums over the threads of a row ---------------------------------------------------------------
+// N sums at once over TPR consecutive lanes (TPR <= 64) or over the whole workgroup of TPR threads, in a fixed order;
+// every thread gets them.  The workgroup form alternates between two LDS buffers, so one barrier per call is enough:
+// a buffer is written again only after the barrier of the call between.
+template <class A, int TPR, int N>
+__device__ inline void row_sums(A (&v)[N], A* lds, int& flip) {
+#pragma unroll
+    for (int m = (TPR < 64 ? TPR : 64) / 2; m > 0; m >>= 1) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], m, 64);
+    }
+    if constexpr (TPR > 64) {
+        constexpr int kWaves = TPR / 64;
+        A* buf = lds + (flip & 1) * kWaves * 2;
+        ++flip;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) buf[(threadIdx.x >> 6) * 2 + n] = v[n];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            A s = buf[n];
+            for (int w = 1; w < kWaves; ++w) s += buf[w * 2 + n];
+            v[n] = s;
+        }
+    }
+}
+
+__device__ inline float inverse_root(float v) { return 1.0f / sqrtf(v); }
+__device__ inline double inverse_root(double v) { return 1.0 / sqrt(v); }
+
+// Which weights, which dropout counter and which row number a row has.
+struct RowPlace {
+    int64_t weight;      // element offset of the row's weights
+    uint32_t row;        // the row's number in the dropout counter
+    uint32_t off[2];
+    bool used;
+};
+template <bool SETS>
+__device__ inline RowPlace place_row(const NormArgs& a, int64_t row) {
+    RowPlace p;
+    p.weight = 0; p.row = (uint32_t)row; p.used = row < a.rows;
+    p.off[0] = p.off[1] = 0;
+    if constexpr (SETS) {
+        if (p.used) {
+            const int set = (int)(row / a.sets.set_rows);
+            p.row = (uint32_t)(row - (int64_t)set * a.sets.set_rows);
+            p.used = (int)p.row < a.sets.set_used[set];
+            p.weight = (int64_t)a.sets.set_index[set] * a.sets.weight_stride;
+            if (a.sets.set_ctr) { p.off[0] = a.sets.set_ctr[2 * set]; p.off[1] = a.sets.set_ctr[2 * set + 1]; }
+        }
+    }
+    return p;
+}
+
+// ---- dropout ----------------------------------------------------------------------------------------
+struct DropShape {
+    int64_t row0;                // first row of the launch
+    uint32_t chunks;             // (row, chunk) pairs of the launch, below 2^31
+    uint32_t per_row;            // chunks of a row
+    uint32_t magic, shift;       // n / per_row = (n * magic) >> shift for every n below 2^31
+    int64_t cols, x_stride, y_stride;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, DropShape s, DropArgs d) {
+    const uint32_t g = blockIdx.x * 256u + threadIdx.x;
+    if (g >= s.chunks) return;
+    const uint32_t r = (uint32_t)(((uint64_t)g * s.magic) >> s.shift), c = g - r * s.per_row;
+    const int64_t row = s.row0 + r, col = (int64_t)c * kChunk;
+    const int count = (int)(s.cols - col < kChunk ? s.cols - col : kChunk);
+    wide_t<T> v[kChunk];
+    load_chunk(x + row * s.x_stride + col, count, v);
+    uint32_t off[2], w[4];
+    drop_offset(d, off);
+    draw_words(d, off, c, (uint32_t)row, w);
+    drop_chunk(d, (wide_t<T>)d.scale, w, v);
+    store_chunk(y + row * s.y_stride + col, count, v);
+}
+
+// ---- layer norm, forward: any width ------------------------------------------------------------------
+// A row is walked three times by TPR threads (mean; spread about it; output); the second and third walk find it in
+// the caches.  The spread is taken about the rounded mean m together with the mean d of what is left, so a mean far
+// from zero costs no digits: variance = mean (h-m)^2 - d^2 and u = ((h-m) - d) r.
+template <class T, int TPR, bool DROP, bool SETS>
+__device__ inline void norm_forward_row(const NormArgs& a, int64_t row, wide_t<T>* lds, int& flip) {
+    using A = wide_t<T>;
+    const int t = threadIdx.x % TPR;
+    RowPlace pl = place_row<SETS>(a, row);
+    if (!pl.used) return;   // the same for all threads of the row, and of the workgroup where it has one row
+    if (DROP && !(SETS && a.sets.set_ctr)) drop_offset(a.drop, pl.off);
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    T* y = static_cast<T*>(a.y) + row * a.y_stride;
+    const A inv = (A)(1.0 / (double)a.cols), scale = (A)a.drop.scale;
+    auto load = [&](int64_t col, int& count, A (&h)[kChunk]) {
+        count = (int)(a.cols - col < kChunk ? a.cols - col : kChunk);
+        load_chunk(x + col, count, h);
+        if constexpr (DROP) {
+            uint32_t w[4];
+            draw_words(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row, w);
+            drop_chunk(a.drop, scale, w, h);
+        }
+    };
+    A s[1] = {0};
+    for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
+        A h[kChunk]; int count;
+        load(col, count, h);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) s[0] += k < count ? h[k] : (A)0;
+    }
+    row_sums<A, TPR, 1>(s, lds, flip);
+    const A m = s[0] * inv;
+    A q[2] = {0, 0};
+    for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
+        A h[kChunk]; int count;
+        load(col, count, h);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) {
+            const A c = k < count ? h[k] - m : (A)0;
+            q[0] += c; q[1] += c * c;
+        }
+    }
+    row_sums<A, TPR, 2>(q, lds, flip);
+    const A d = q[0] * inv;
+    A var = q[1] * inv - d * d;
+    var = var < 0 ? (A)0 : var;   // keeps NaN
+    const A r = inverse_root(var + (A)a.eps);
+    if (t == 0 && a.mean) { static_cast<A*>(a.mean)[row] = m + d; static_cast<A*>(a.rstd)[row] = r; }
+    const T* weight = a.weight ? static_cast<const T*>(a.weight) + pl.weight : nullptr;
+    const T* bias = a.bias ? static_cast<const T*>(a.bias) + pl.weight : nullptr;
+    for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
+        A h[kChunk], g[kChunk], b[kChunk]; int count;
+        load(col, count, h);
+        if (weight) load_chunk(weight + col, count, g);
+        if (bias) load_chunk(bias + col, count, b);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) {
+            const A u = ((h[k] - m) - d) * r;
+            h[k] = (weight ? u * g[k] : u) + (bias ? b[k] : (A)0);
+        }
+        store_chunk(y + col, count, h);
+    }
+}
+
+// A launch holds at most kMaxBlocks workgroups (a grid has fewer than 2^32 threads): they walk on over the rows.
+constexpr int64_t kMaxBlocks = (int64_t)1 << 20;
+
+template <class T, int TPR, bool DROP, bool SETS>
+__global__ __launch_bounds__(256) void norm_forward_walk_kernel(NormArgs a) {
+    __shared__ wide_t<T> lds[TPR > 64 ? 2 * (TPR / 64) * 2 : 1];
+    int flip = 0;
+    constexpr int kRows = 256 / TPR;
+    for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * kRows)
+        norm_forward_row<T, TPR, DROP, SETS>(a, row, lds, flip);
+}
+
+// ---- layer norm, backward: any width -------------------------------------------------------------------
+// One launch of two kinds of workgroups that do not wait for each other.  The first row_blocks take rows and write
+// dx, TPR threads a row, in two walks (the two means; the result).  The others take columns, 32 of them and
+// seg_rows rows each, and form sums of dy u and dy: 4 threads side by side, 64 rows at a time, then the 64 sums of
+// every column in a fixed order.  With one segment they are the gradients, else partial sums for
+// norm_reduce_kernel.
+constexpr int kTileCols = 32, kTileSlots = 64;
+
+struct SplitShape {
+    int64_t row_blocks, col_tiles, segs, seg_rows;
+};
+
+template <class T, bool DROP, bool SETS>
+__device__ inline void column_sums(const NormArgs& a, const SplitShape& sh, int64_t block, wide_t<T>* lds) {
+    using A = wide_t<T>;
+    const int64_t tile = block % sh.col_tiles, seg = block / sh.col_tiles;   // SETS: a segment is a set
+    const int64_t first = seg * sh.seg_rows;
+    int64_t last = first + sh.seg_rows < a.rows ? first + sh.seg_rows : a.rows;
+    if constexpr (SETS) last = first + a.sets.set_used[seg] < last ? first + a.sets.set_used[seg] : last;
+    const int lane = threadIdx.x % 4, slot = threadIdx.x / 4;
+    const int64_t col = tile * kTileCols + lane * kChunk;
+    const int64_t room = a.cols - col;
+    const int count = (int)(room < 0 ? 0 : room < kChunk ? room : kChunk);
+    uint32_t off[2] = {0, 0};
+    if constexpr (DROP) drop_offset(a.drop, off);
+    if (SETS && a.sets.set_ctr) { off[0] = a.sets.set_ctr[2 * seg]; off[1] = a.sets.set_ctr[2 * seg + 1]; }
+    const A scale = (A)a.drop.scale;
+    A gw[kChunk], gb[kChunk];
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) gw[k] = gb[k] = 0;
+    if (count > 0) {
+        for (int64_t row = first + slot; row < last; row += kTileSlots) {
+            A h[kChunk], dy[kChunk];
+            load_chunk(static_cast<const T*>(a.x) + row * a.x_stride + col, count, h);
+            load_chunk(static_cast<const T*>(a.dy) + row * a.dy_stride + col, count, dy);
+            const A m = static_cast<const A*>(a.mean)[row], r = static_cast<const A*>(a.rstd)[row];
+            if constexpr (DROP) {
+                uint32_t w[4];
+                draw_words(a.drop, off, (uint32_t)(col / kChunk), (uint32_t)(SETS ? row - first : row), w);
+                drop_chunk(a.drop, scale, w, h);
+            }
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) {
+                gw[k] += dy[k] * ((h[k] - m) * r);
+                gb[k] += dy[k];
+            }
+        }
+    }
+    // [2][slot][column]: 64 threads sum the 32 columns of both
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+        lds[slot * kTileCols + lane * kChunk + k] = gw[k];
+        lds[(kTileSlots + slot) * kTileCols + lane * kChunk + k] = gb[k];
+    }
+    __syncthreads();
+    const int which = threadIdx.x / kTileCols, c = threadIdx.x % kTileCols;
+    if (which < 2 && tile * kTileCols + c < a.cols) {
+        A part[4] = {0, 0, 0, 0};
+        for (int k = 0; k < kTileSlots; k += 4) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) part[u] += lds[(which * kTileSlots + k + u) * kTileCols + c];
+        }
+        const A total = (part[0] + part[1]) + (part[2] + part[3]);
+        const int64_t at = tile * kTileCols + c;
+        if (SETS || sh.segs == 1) {
+            T* out = static_cast<T*>(which ? a.dbias : a.dweight);
+            if (out) out[seg * a.cols + at] = (T)total;
+        } else {
+            static_cast<A*>(a.workspace)[(seg * 2 + which) * a.cols + at] = total;
+        }
+    }
+}
+
+template <class T, int TPR, bool DROP, bool SETS>
+__device__ inline void norm_backward_row(const NormArgs& a, int64_t row, wide_t<T>* lds, int& flip) {
+    using A = wide_t<T>;
+    const int t = threadIdx.x % TPR;
+    RowPlace pl = place_row<SETS>(a, row);
+    if (!pl.used) return;
+    if (DROP && !(SETS && a.sets.set_ctr)) drop_offset(a.drop, pl.off);
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
+    T* dx = static_cast<T*>(a.dx) + row * a.y_stride;
+    const T* weight = a.weight ? static_cast<const T*>(a.weight) + pl.weight : nullptr;
+    const A inv = (A)(1.0 / (double)a.cols), scale = (A)a.drop.scale;
+    const A m = static_cast<const A*>(a.mean)[row], r = static_cast<const A*>(a.rstd)[row];
+    auto load = [&](int64_t col, int& count, A (&u)[kChunk], A (&g)[kChunk], uint32_t (&w)[4]) {
+        count = (int)(a.cols - col < kChunk ? a.cols - col : kChunk);
+        load_chunk(x + col, count, u);
+        load_chunk(dy + col, count, g);
+        if constexpr (DROP) {
+            draw_words(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row, w);
+            drop_chunk(a.drop, scale, w, u);
+        }
+        A gain[kChunk];
+        if (weight) load_chunk(weight + col, count, gain);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) {
+            u[k] = (u[k] - m) * r;
+            if (weight) g[k] *= gain[k];
+        }
+    };
+    A s[2] = {0, 0};
+    for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
+        A u[kChunk], g[kChunk]; uint32_t w[4]; int count;
+        load(col, count, u, g, w);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) {
+            s[0] += k < count ? g[k] : (A)0;
+            s[1] += k < count ? g[k] * u[k] : (A)0;
+        }
+    }
+    row_sums<A, TPR, 2>(s, lds, flip);
+    const A c1 = s[0] * inv, c2 = s[1] * inv;
+    for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
+        A u[kChunk], g[kChunk]; uint32_t w[4]; int count;
+        load(col, count, u, g, w);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) g[k] = ((g[k] - c1) - u[k] * c2) * r;
+        if constexpr (DROP) drop_chunk(a.drop, scale, w, g);
+        store_chunk(dx + col, count, g);
+    }
+}
+
+template <class T, int TPR, bool DROP, bool SETS>
+__global__ __launch_bounds__(256) void norm_backward_split_kernel(NormArgs a, SplitShape sh) {
+    using A = wide_t<T>;
+    __shared__ A lds[2 * kTileSlots * kTileCols];
+    if ((int64_t)blockIdx.x < sh.row_blocks) {
+        int flip = 0;
+        constexpr int kRows = 256 / TPR;
+        for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; row < a.rows; row += sh.row_blocks * kRows)
+            norm_backward_row<T, TPR, DROP, SETS>(a, row, lds, flip);
+    } else {
+        const int64_t stride = (int64_t)gridDim.x - sh.row_blocks;
+        for (int64_t b = (int64_t)blockIdx.x - sh.row_blocks; b < sh.col_tiles * sh.segs; b += stride) {
+            column_sums<T, DROP, SETS>(a, sh, b, lds);
+            __syncthreads();   // the sums are read before the next tile's are written
+        }
+    }
+}
+
+// Sums the partial rows of the two gradients: 16 columns and 64 rows at a time, then the 64 sums in a fixed order.
+template <class T>
+__global__ __launch_bounds__(1024) void norm_reduce_kernel(const wide_t<T>* __restrict__ part, int64_t parts, int64_t cols,
+                                                           T* dweight, T* dbias) {
+    using A = wide_t<T>;
+    __shared__ A lds[64][17];
+    const int lane = threadIdx.x % 16, slot = threadIdx.x / 16;
+    const int64_t at = (int64_t)blockIdx.x * 16 + lane;   // over [2][cols]
+    A s = 0;
+    if (at < 2 * cols) {
+#pragma unroll 8
+        for (int64_t p = slot; p < parts; p += 64) s += part[p * 2 * cols + at];
+    }
+    lds[slot][lane] = s;
+    __syncthreads();
+    for (int half = 32; half > 0; half >>= 1) {
+        if (slot < half) lds[slot][lane] += lds[slot + half][lane];
+        __syncthreads();
+    }
+    if (slot == 0 && at < 2 * cols) {
+        T* out = at < cols ? dweight : dbias;
+        if (out) out[at < cols ? at : at - cols] = (T)lds[0][lane];
+    }
+}
+
+// dweight and dbias of no rows at all
+template <class T>
+__global__ __launch_bounds__(256) void norm_zero_kernel(T* dweight, T* dbias, int64_t cols) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    if (dweight) dweight[c] = (T)0;
+    if (dbias) dbias[c] = (T)0;
+}
+
+// ---- launching --------------------------------------------------------------------------------------
+// Calls f with a value of the element type.
+template <class F>
+auto with_type(LayerType type, F f) {
+    switch (type) {
+        case kF64: return f(double{});
+        case kF32: return f(float{});
+        case kBF16: return f(__bf16{});
+        default: return f(_Float16{});
+    }
+}
+template <class F>
+auto with_flag(bool on, F f) {
+    return on ? f(std::true_type{}) : f(std::false_type{});
+}
+
+// Rows of one column workgroup: as many as keep its walk short; more rows than that become segments.
+constexpr int64_t kSegRows = 1024;
+
+SplitShape split_shape(const NormArgs& a, int tpr) {
+    SplitShape sh{};
+    sh.row_blocks = a.dx ? std::min((a.rows + 256 / tpr - 1) / (256 / tpr), kMaxBlocks) : 0;
+    sh.col_tiles = (a.cols + kTileCols - 1) / kTileCols;
+    if (a.sets.count) {
+        sh.segs = a.sets.count; sh.seg_rows = a.sets.set_rows;
+    } else {
+        sh.segs = (a.rows + kSegRows - 1) / kSegRows; sh.seg_rows = kSegRows;
+    }
+    return sh;
+}
+
+}  // namespace
+
+DropArgs make_drop(double p, int64_t seed, int64_t offset, const int64_t* offset_dev) {
+    DropArgs d{};
+    d.threshold = (uint32_t)std::nearbyint(p * 65536.0);
+    d.scale = d.threshold < 65536 ? 65536.0 / (65536.0 - d.threshold) : 0.0;
+    d.key[0] = (uint32_t)(uint64_t)seed; d.key[1] = (uint32_t)((uint64_t)seed >> 32);
+    d.offset[0] = (uint32_t)(uint64_t)offset; d.offset[1] = (uint32_t)((uint64_t)offset >> 32);
+    d.offset_dev = offset_dev;
+    return d;
+}
+
+hipError_t launch_dropout(LayerType type, int64_t rows, int64_t cols, int64_t x_stride, int64_t y_stride, const void* x,
+                          void* y, const DropArgs& drop, hipStream_t s) {
+    DropShape sh{};
+    sh.cols = cols; sh.x_stride = x_stride; sh.y_stride = y_stride;
+    sh.per_row = (uint32_t)((cols + kChunk - 1) / kChunk);
+    // with l = ceil(log2 per_row) and magic = ceil(2^(31+l) / per_row) the quotient is exact below 2^31, and the
+    // magic number stays below 2^32
+    int l = 0;
+    while (((uint64_t)1 << l) < sh.per_row) ++l;
+    sh.shift = 31 + l;
+    sh.magic = (uint32_t)((((uint64_t)1 << (31 + l)) + sh.per_row - 1) / sh.per_row);
+    const int64_t per_launch = ((int64_t)1 << 31) / sh.per_row - 1;   // rows: at least 7, for fewer than 2^28 chunks a row
+    for (int64_t r = 0; r < rows; r += per_launch) {
+        const int64_t n = rows - r < per_launch ? rows - r : per_launch;
+        sh.row0 = r;
+        sh.chunks = (uint32_t)(n * sh.per_row);
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            hipLaunchKernelGGL(dropout_kernel<T>, dim3((sh.chunks + 255) / 256), dim3(256), 0, s, static_cast<const T*>(x),
+                               static_cast<T*>(y), sh, drop);
+        });
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_norm_forward(LayerType type, const NormArgs& a, hipStream_t s) {
+    if (a.rows == 0) return hipSuccess;
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        with_flag(a.drop.threshold != 0, [&](auto drop) {
+            constexpr bool D = decltype(drop)::value;
+            if (a.cols <= 2048)
+                hipLaunchKernelGGL((norm_forward_walk_kernel<T, 64, D, false>), dim3((unsigned)std::min((a.rows + 3) / 4, kMaxBlocks)), dim3(256), 0, s, a);
+            else
+                hipLaunchKernelGGL((norm_forward_walk_kernel<T, 256, D, false>), dim3((unsigned)std::min(a.rows, kMaxBlocks)), dim3(256), 0, s, a);
+        });
+    });
+    return hipGetLastError();
+}
+
+size_t norm_backward_workspace(LayerType type, int64_t rows, int64_t cols) {
+    const int64_t segs = (rows + kSegRows - 1) / kSegRows;
+    return segs > 1 ? (size_t)segs * 2 * cols * (type == kF64 ? 8 : 4) : 0;
+}
+
+hipError_t launch_norm_backward(LayerType type, const NormArgs& a, hipStream_t s) {
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (a.rows == 0) {
+            if (a.dweight || a.dbias)
+                hipLaunchKernelGGL(norm_zero_kernel<T>, dim3((unsigned)((a.cols + 255) / 256)), dim3(256), 0, s,
+                                   static_cast<T*>(a.dweight), static_cast<T*>(a.dbias), a.cols);
+            return;
+        }
+        const bool wide = a.cols > 2048;
+        SplitShape sh = split_shape(a, wide ? 256 : 64);
+        const int64_t col_blocks = a.dweight || a.dbias ? std::min(sh.col_tiles * sh.segs, kMaxBlocks) : 0;
+        if (sh.row_blocks + col_blocks == 0) return;
+        const dim3 grid((unsigned)(sh.row_blocks + col_blocks));
+        with_flag(a.drop.threshold != 0, [&](auto drop) {
+            constexpr bool D = decltype(drop)::value;
+            if (wide) hipLaunchKernelGGL((norm_backward_split_kernel<T, 256, D, false>), grid, dim3(256), 0, s, a, sh);
+            else hipLaunchKernelGGL((norm_backward_split_kernel<T, 64, D, false>), grid, dim3(256), 0, s, a, sh);
+        });
+        if (col_blocks && sh.segs > 1)
+            hipLaunchKernelGGL(norm_reduce_kernel<T>, dim3((unsigned)((2 * a.cols + 15) / 16)), dim3(1024), 0, s,
+                               static_cast<const wide_t<T>*>(a.workspace), sh.segs, a.cols, static_cast<T*>(a.dweight),
+                               static_cast<T*>(a.dbias));
+    });
+    return hipGetLastError();
+}
+
+// ---- C entry points ------------------------------------------------------------------------------------
+namespace {
+
+// Makes the call's device current and puts the caller's back at the end.
+struct DeviceScope {
+    int before = -1;
+    bool changed = false;
+    int32_t enter(int device) {
+        if (hipGetDevice(&before) != hipSuccess)
+            return fail(EPI_ERR_DEVICE, "no HIP device available: the engine has no CPU fallback");
+        if (device == before) return EPI_OK;
+        if (int32_t rc = use_device(device)) return rc;
+        changed = true;
+        return EPI_OK;
+    }
+    ~DeviceScope() { if (changed) (void)hipSetDevice(before); }
+};
+
+// [lo, hi) in bytes of `rows` rows of `cols` elements
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    if (!a || !b) return false;
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    return p < q + (uintptr_t)b_bytes && q < p + (uintptr_t)a_bytes;
+}
+
+struct Extent {
+    int64_t size;   // bytes of an element
+    int64_t plane(int64_t rows, int64_t cols, int64_t stride) const { return rows ? ((rows - 1) * stride + cols) * size : 0; }
+};
+
+int32_t check_desc(const char* who, const epi_layer_desc* d, Extent* e) {
+    if (!d) return fail(EPI_ERR_BAD_ARGUMENT, "%s: null descriptor", who);
+    if (d->dtype < EPI_F64 || d->dtype > EPI_F16) return fail(EPI_ERR_BAD_ARGUMENT, "%s: dtype %d outside [0,3]", who, d->dtype);
+    e->size = d->dtype == EPI_F64 ? 8 : d->dtype == EPI_F32 ? 4 : 2;
+    if (d->rows < 0 || d->cols < 1) return fail(EPI_ERR_BAD_ARGUMENT, "%s: %lld rows of %lld columns", who, (long long)d->rows, (long long)d->cols);
+    if (d->rows >= (int64_t)1 << 31 || d->cols >= (int64_t)1 << 31)
+        return fail(EPI_ERR_UNSUPPORTED, "%s: %lld rows of %lld columns: both must be below 2^31", who, (long long)d->rows, (long long)d->cols);
+    if (!(d->dropout >= 0.0 && d->dropout <= 1.0)) return fail(EPI_ERR_BAD_ARGUMENT, "%s: dropout %g outside [0,1]", who, d->dropout);
+    if (reinterpret_cast<uintptr_t>(d->offset_dev) % 8) return fail(EPI_ERR_BAD_ARGUMENT, "%s: offset_dev is not aligned", who);
+    return EPI_OK;
+}
+
+int32_t check_plane(const char* who, const char* name, const void* p, int64_t rows, int64_t cols, int64_t stride, int64_t size, bool written) {
+    if (rows == 0) return EPI_OK;
+    if (!p) return fail(EPI_ERR_BAD_ARGUMENT, "%s: %s is null", who, name);
+    if (reinterpret_cast<uintptr_t>(p) % size) return fail(EPI_ERR_BAD_ARGUMENT, "%s: %s is not aligned to its elements", who, name);
+    if (rows > 1 && (stride < 0 || (written && stride < cols) || stride >= (int64_t)1 << 40))
+        return fail(EPI_ERR_BAD_ARGUMENT, "%s: %s has a row stride of %lld for %lld columns", who, name, (long long)stride, (long long)cols);
+    return EPI_OK;
+}
+
+int32_t check_vector(const char* who, const char* name, const void* p, int64_t size) {
+    if (reinterpret_cast<uintptr_t>(p) % size) return fail(EPI_ERR_BAD_ARGUMENT, "%s: %s is not aligned to its elements", who, name);
+    return EPI_OK;
+}
+
+}  // namespace
+}  // namespace epi
+
+using namespace epi;
+
+EPI_API int32_t epi_dropout(const epi_layer_desc* d, const void* x, void* y, void* stream) {
+    const char* who = "dropout";
+    Extent e{};
+    if (int32_t rc = check_desc(who, d, &e)) return rc;
+    if (int32_t rc = check_plane(who, "x", x, d->rows, d->cols, d->x_stride, e.size, false)) return rc;
+    if (int32_t rc = check_plane(who, "y", y, d->rows, d->cols, d->y_stride, e.size, true)) return rc;
+    const bool in_place = x == y && (d->rows < 2 || d->x_stride == d->y_stride);
+    if (!in_place && overlap(x, e.plane(d->rows, d->cols, d->x_stride), y, e.plane(d->rows, d->cols, d->y_stride)))
+        return fail(EPI_ERR_BAD_ARGUMENT, "dropout: x and y overlap without being the same rows");
+    DeviceScope dev;
+    if (int32_t rc = dev.enter(d->device)) return rc;
+    if (d->rows == 0) return EPI_OK;
+    HIP_TRY(launch_dropout((LayerType)d->dtype, d->rows, d->cols, d->x_stride, d->y_stride, x, y,
+                           make_drop(d->dropout, d->seed, d->offset, d->offset_dev), static_cast<hipStream_t>(stream)));
+    return EPI_OK;
+}
+
+EPI_API int32_t epi_layer_norm_forward(const epi_layer_desc* d, const void* x, const void* weight, const void* bias, void* y,
+                                       void* mean, void* rstd, void* stream) {
+    const char* who = "layer_norm_forward";
+    Extent e{};
+    if (int32_t rc = check_desc(who, d, &e)) return rc;
+    const int64_t wide = e.size == 8 ? 8 : 4, vec = d->cols * e.size, stat = d->rows * wide;
+    if (!(d->eps >= 0.0)) return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_forward: eps %g is negative", d->eps);
+    if (int32_t rc = check_plane(who, "x", x, d->rows, d->cols, d->x_stride, e.size, false)) return rc;
+    if (int32_t rc = check_plane(who, "y", y, d->rows, d->cols, d->y_stride, e.size, true)) return rc;
+    if (int32_t rc = check_vector(who, "weight", weight, e.size)) return rc;
+    if (int32_t rc = check_vector(who, "bias", bias, e.size)) return rc;
+    if (int32_t rc = check_vector(who, "mean", mean, wide)) return rc;
+    if (int32_t rc = check_vector(who, "rstd", rstd, wide)) return rc;
+    if (!mean != !rstd) return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_forward: mean and rstd are asked for together");
+    const int64_t ny = e.plane(d->rows, d->cols, d->y_stride), nx = e.plane(d->rows, d->cols, d->x_stride);
+    const bool in_place = x == y && (d->rows < 2 || d->x_stride == d->y_stride);
+    if ((!in_place && overlap(x, nx, y, ny)) || overlap(y, ny, weight, vec) || overlap(y, ny, bias, vec) ||
+        overlap(y, ny, mean, stat) || overlap(y, ny, rstd, stat) || overlap(x, nx, mean, stat) || overlap(x, nx, rstd, stat) ||
+        overlap(mean, stat, rstd, stat) || overlap(mean, stat, weight, vec) || overlap(mean, stat, bias, vec) ||
+        overlap(rstd, stat, weight, vec) || overlap(rstd, stat, bias, vec))
+        return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_forward: an output overlaps another array (y may be x itself)");
+    DeviceScope dev;
+    if (int32_t rc = dev.enter(d->device)) return rc;
+    NormArgs a{};
+    a.rows = d->rows; a.cols = d->cols; a.x_stride = d->x_stride; a.y_stride = d->y_stride;
+    a.x = x; a.weight = weight; a.bias = bias; a.y = y; a.mean = mean; a.rstd = rstd; a.eps = d->eps;
+    a.drop = make_drop(d->dropout, d->seed, d->offset, d->offset_dev);
+    HIP_TRY(launch_norm_forward((LayerType)d->dtype, a, static_cast<hipStream_t>(stream)));
+    return EPI_OK;
+}
+
+EPI_API int32_t epi_layer_norm_backward_workspace(const epi_layer_desc* d, size_t* bytes) {
+    Extent e{};
+    if (int32_t rc = check_desc("layer_norm_backward_workspace", d, &e)) return rc;
+    if (!bytes) return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_backward_workspace: null argument");
+    *bytes = norm_backward_workspace((LayerType)d->dtype, d->rows, d->cols);
+    return EPI_OK;
+}
+
+EPI_API int32_t epi_layer_norm_backward(const epi_layer_desc* d, const void* x, const void* dy, const void* weight,
+                                        const void* mean, const void* rstd, void* dx, void* dweight, void* dbias,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "layer_norm_backward";
+    Extent e{};
+    if (int32_t rc = check_desc(who, d, &e)) return rc;
+    const int64_t wide = e.size == 8 ? 8 : 4, vec = d->cols * e.size, stat = d->rows * wide;
+    if (int32_t rc = check_plane(who, "x", x, d->rows, d->cols, d->x_stride, e.size, false)) return rc;
+    if (int32_t rc = check_plane(who, "dy", dy, d->rows, d->cols, d->dy_stride, e.size, false)) return rc;
+    if (dx) {
+        if (int32_t rc = check_plane(who, "dx", dx, d->rows, d->cols, d->y_stride, e.size, true)) return rc;
+    }
+    if (d->rows && (!mean || !rstd)) return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_backward: mean or rstd is null");
+    const struct { const char* name; const void* p; int64_t size; } vectors[] = {
+        {"weight", weight, e.size}, {"mean", mean, wide}, {"rstd", rstd, wide}, {"dweight", dweight, e.size},
+        {"dbias", dbias, e.size}, {"workspace", workspace, wide}};
+    for (const auto& v : vectors)
+        if (int32_t rc = check_vector(who, v.name, v.p, v.size)) return rc;
+    size_t need = 0;
+    if (dweight || dbias) need = norm_backward_workspace((LayerType)d->dtype, d->rows, d->cols);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_backward: a workspace of %zu bytes is needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    const struct { const void* p; int64_t n; } in[] = {
+        {x, e.plane(d->rows, d->cols, d->x_stride)}, {dy, e.plane(d->rows, d->cols, d->dy_stride)}, {weight, vec}, {mean, stat}, {rstd, stat}};
+    const struct { const void* p; int64_t n; } out[] = {
+        {dx, e.plane(d->rows, d->cols, d->y_stride)}, {dweight, vec}, {dbias, vec}, {workspace, (int64_t)need}};
+    for (int i = 0; i < 4; ++i) {
+        for (const auto& j : in)
+            if (overlap(out[i].p, out[i].n, j.p, j.n)) return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_backward: an output overlaps an input");
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i].p, out[i].n, out[j].p, out[j].n)) return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_backward: two outputs overlap");
+    }
+    DeviceScope dev;
+    if (int32_t rc = dev.enter(d->device)) return rc;
+    NormArgs a{};
+    a.rows = d->rows; a.cols = d->cols; a.x_stride = d->x_stride; a.y_stride = d->y_stride; a.dy_stride = d->dy_stride;
+    a.x = x; a.dy = dy; a.weight = weight; a.mean = const_cast<void*>(mean); a.rstd = const_cast<void*>(rstd);
+    a.dx = dx; a.dweight = dweight; a.dbias = dbias; a.workspace = workspace;
+    a.drop = make_drop(d->dropout, d->seed, d->offset, d->offset_dev);
+    HIP_TRY(launch_norm_backward((LayerType)d->dtype, a, static_cast<hipStream_t>(stream)));
+    return EPI_OK;
+}

@@ -407,6 +407,54 @@ int32_t epi_agents_set_weights(epi_agents *g, int32_t agent, int32_t target, con
 int32_t epi_agents_set_timing(epi_agents *g, int32_t on);
 int32_t epi_agents_kernel_time(epi_agents *g, double *total_ms, int64_t *learn_calls, int64_t *samples);
 
+/* ---- Layers of a network on the device (no counterpart in the reference) ----------------------------
+ * What a Q-network that replays its buffer often is regularised with, as operators on device memory: dropout from a
+ * counter-based generator, whose mask is never stored, and layer normalisation, forward and backward, separately or in
+ * one pass (dropout of the input first).  Every call only enqueues kernels on `stream` (a hipStream_t, NULL = the
+ * default stream) of device d->device: it allocates nothing, keeps nothing and never waits, so it can be captured.
+ * The caller's current device is left as it was.  All array arguments are device memory there, aligned to their
+ * elements; rows are x_stride, y_stride and dy_stride elements apart (any stride >= 0 for what is read, at least
+ * `cols` for what is written), columns lie next to each other.
+ *
+ * dropout: t = d->dropout in units of 2^-16, rounded (halves to even).  Column c of row r is dropped when its draw of
+ * 16 bits is below t, and multiplied by 65536 / (65536 - t) otherwise; a dropped value gives 0 whatever it was.  The
+ * draws are half-words c % 8 (the low half of a word first) of the four words that Philox4x32-10 gives for the key
+ * d->seed and the counter (c / 8, r, low word, high word of offset), offset = d->offset + *d->offset_dev, all as 64-bit
+ * two's complement numbers.  The same seed, offset and shape give the same mask on every call, which is how the
+ * backward pass drops what the forward pass did; calls that are to draw independently take different offsets. */
+typedef enum epi_dtype { EPI_F64 = 0, EPI_F32 = 1, EPI_BF16 = 2, EPI_F16 = 3 } epi_dtype;
+
+typedef struct epi_layer_desc {
+    int64_t rows, cols;         /* 0 <= rows < 2^31, 1 <= cols < 2^31 */
+    int64_t x_stride;           /* of x */
+    int64_t y_stride;           /* of y, or dx in a backward call */
+    int64_t dy_stride;          /* of dy (epi_layer_norm_backward only) */
+    double eps;                 /* >= 0 (layer norm only) */
+    double dropout;             /* 0 .. 1 */
+    int64_t seed, offset;       /* of the dropout's generator */
+    const int64_t *offset_dev;  /* NULL, or one number in device memory that the kernels add to offset when they run:
+                                 * a captured graph draws anew on every replay if the program changes it in between */
+    int32_t dtype;              /* an epi_dtype: of all arrays but mean and rstd */
+    int32_t device;             /* HIP device ordinal */
+} epi_layer_desc;
+
+/* y = dropout(x).  The gradient is the same map: epi_dropout of dy with the same descriptor gives dx.  y may be x. */
+int32_t epi_dropout(const epi_layer_desc *d, const void *x, void *y, void *stream);
+/* y = (h - m) * r * weight + bias per row, with h = x, or dropout(x) where d->dropout > 0; m = mean of h,
+ * r = 1 / sqrt(mean (h - m)^2 + eps).  weight[cols] and bias[cols] may be NULL (ones, zeros).  mean[rows] and
+ * rstd[rows] = m and r for the backward pass, doubles for EPI_F64 and floats otherwise; both may be NULL.  Sums and
+ * everything between load and store are in the type of mean; y is rounded once.  y may be x. */
+int32_t epi_layer_norm_forward(const epi_layer_desc *d, const void *x, const void *weight, const void *bias, void *y,
+                               void *mean, void *rstd, void *stream);
+/* Bytes of workspace that epi_layer_norm_backward needs for a descriptor's dtype, rows and cols (may be 0). */
+int32_t epi_layer_norm_backward_workspace(const epi_layer_desc *d, size_t *bytes);
+/* dx[rows][cols], dweight[cols] and dbias[cols] (each may be NULL) from x, dy, weight (NULL = ones) and the mean and
+ * rstd of the forward pass, with the same dropout, seed and offset.  Sums over the rows are taken in a fixed order in
+ * the type of mean and rounded once: the same call gives the same bits.  No output may overlap another array. */
+int32_t epi_layer_norm_backward(const epi_layer_desc *d, const void *x, const void *dy, const void *weight,
+                                const void *mean, const void *rstd, void *dx, void *dweight, void *dbias,
+                                void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

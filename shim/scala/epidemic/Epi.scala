@@ -83,6 +83,10 @@ object Epi {
   val agentsSetWeights = fn("epi_agents_set_weights", JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
   val agentsSetTiming = fn("epi_agents_set_timing", JAVA_INT, ADDRESS, JAVA_INT)
   val agentsKernelTime = fn("epi_agents_kernel_time", JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
+  val dropout = fn("epi_dropout", JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
+  val layerNormForward = fn("epi_layer_norm_forward", JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
+  val layerNormBackwardWorkspace = fn("epi_layer_norm_backward_workspace", JAVA_INT, ADDRESS, ADDRESS)
+  val layerNormBackward = fn("epi_layer_norm_backward", JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, JAVA_LONG, ADDRESS)
 
   // ---- struct layouts of include/epi.h (java.lang.foreign inserts no padding: it is spelled out)
   val PROFILE: StructLayout = MemoryLayout.structLayout(   // 72 bytes
@@ -184,6 +188,19 @@ object Epi {
     JAVA_INT.withName("v"),
     JAVA_INT.withName("t"),
     JAVA_DOUBLE.withName("hosp_cap"))
+  val LAYER_DESC: StructLayout = MemoryLayout.structLayout(   // 88 bytes
+    JAVA_LONG.withName("rows"),
+    JAVA_LONG.withName("cols"),
+    JAVA_LONG.withName("x_stride"),
+    JAVA_LONG.withName("y_stride"),
+    JAVA_LONG.withName("dy_stride"),
+    JAVA_DOUBLE.withName("eps"),
+    JAVA_DOUBLE.withName("dropout"),
+    JAVA_LONG.withName("seed"),
+    JAVA_LONG.withName("offset"),
+    ADDRESS.withName("offset_dev"),
+    JAVA_INT.withName("dtype"),
+    JAVA_INT.withName("device"))
 
   // ---- status handling ---------------------------------------------------------------------------------------
   val OK = 0; val BAD_ARGUMENT = 1; val DEVICE = 2; val LOCAL_MASS = 3; val WORLD_MASS = 4; val ASSERT_STATE = 5
