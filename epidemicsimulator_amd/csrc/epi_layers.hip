@@ -20,6 +20,8 @@
 
 #define EPI_API extern "C" __attribute__((visibility("default")))
 
+#pragma clang fp contract(fast)   // products go into sums unrounded
+
 namespace epi {
 namespace {
 
@@ -30,33 +32,151 @@ template <> struct Wide<double> { using type = double; };
 template <class T> using wide_t = typename Wide<T>::type;
 
 // ---- chunks of eight columns ------------------------------------------------------------------
-// Rows of odd widths start at any multiple of the element's size, so the vectors are declared with the element's
-// alignment: the hardware takes 16-byte accesses at any address, and rows that do start at 16 bytes lose nothing.
-template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Chunk { T v[kChunk]; };
+// A chunk on its way is whole 32-bit words: nothing has to wait for it before its first use.  Rows of odd widths
+// start at any multiple of the element's size, so accesses are declared with the element's alignment: the hardware
+// takes 16 bytes at any address, and rows that do start at 16 bytes lose nothing.  The last chunk of a row that is no
+// multiple of eight is put together from a part of four, of two and of one element.
+template <class T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Part { uint32_t w[N]; };
+template <class T> struct Raw {
+    static constexpr int kWords = kChunk * sizeof(T) / 4;
+    uint32_t w[kWords];
+};
 
-template <class T>
-__device__ inline void load_chunk(const T* p, int count, wide_t<T> (&out)[kChunk]) {
-    if (count >= kChunk) {
-        const Chunk<T> c = *reinterpret_cast<const Chunk<T>*>(p);
+// the words of N elements (N even, or elements of 4 bytes and more)
+template <class T, int N>
+__device__ inline void fetch_part(const T* p, uint32_t* w) {
+    constexpr int W = N * sizeof(T) / 4;
+    const Part<T, W> v = *reinterpret_cast<const Part<T, W>*>(p);
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) out[k] = (wide_t<T>)c.v[k];
-    } else {
+    for (int i = 0; i < W; ++i) w[i] = v.w[i];
+}
+template <class T, int N>
+__device__ inline void put_part(T* p, const uint32_t* w) {
+    constexpr int W = N * sizeof(T) / 4;
+    Part<T, W> v;
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) out[k] = k < count ? (wide_t<T>)p[k] : (wide_t<T>)0;
-    }
+    for (int i = 0; i < W; ++i) v.w[i] = w[i];
+    *reinterpret_cast<Part<T, W>*>(p) = v;
 }
 
 template <class T>
-__device__ inline void store_chunk(T* p, int count, const wide_t<T> (&in)[kChunk]) {
+__device__ inline void fetch_chunk(const T* p, int count, Raw<T>& c) {
+    constexpr int W = Raw<T>::kWords;
     if (count >= kChunk) {
-        Chunk<T> c;
+        fetch_part<T, kChunk>(p, c.w);
+        return;
+    }
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) c.v[k] = (T)in[k];
-        *reinterpret_cast<Chunk<T>*>(p) = c;
-    } else {
+    for (int i = 0; i < W; ++i) c.w[i] = 0;
+    if (count <= 0) return;
+    // from the back: what is there moves up by the part put before it
+    if (count & 1) {
+        const T* q = p + (count & 6);
+        if constexpr (sizeof(T) == 2) c.w[0] = *reinterpret_cast<const uint16_t*>(q);
+        else fetch_part<T, 1>(q, c.w);
+    }
+    if (count & 2) {
+        uint32_t v[W / 4];
+        fetch_part<T, 2>(p + (count & 4), v);
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k)
-            if (k < count) p[k] = (T)in[k];
+        for (int i = W / 2 - 1; i >= W / 4; --i) c.w[i] = c.w[i - W / 4];
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) c.w[i] = v[i];
+    }
+    if (count & 4) {
+        uint32_t v[W / 2];
+        fetch_part<T, 4>(p, v);
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) { c.w[i + W / 2] = c.w[i]; c.w[i] = v[i]; }
+    }
+}
+template <class T>
+__device__ inline void put_chunk(T* p, int count, Raw<T> c) {
+    constexpr int W = Raw<T>::kWords;
+    if (count >= kChunk) {
+        put_part<T, kChunk>(p, c.w);
+        return;
+    }
+    if (count <= 0) return;
+    if (count & 4) {
+        put_part<T, 4>(p, c.w);
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) c.w[i] = c.w[i + W / 2];
+        p += 4;
+    }
+    if (count & 2) {
+        put_part<T, 2>(p, c.w);
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) c.w[i] = c.w[i + W / 4];
+        p += 2;
+    }
+    if (count & 1) {
+        if constexpr (sizeof(T) == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)c.w[0];
+        else put_part<T, 1>(p, c.w);
+    }
+}
+
+template <class T> struct Pair { T lo, hi; };
+template <class T>
+__device__ inline void widen_chunk(const Raw<T>& c, wide_t<T> (&out)[kChunk]) {
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+        if constexpr (std::is_same_v<T, __bf16>) {
+            out[k] = __builtin_bit_cast(float, (k & 1) ? c.w[k / 2] & 0xffff0000u : c.w[k / 2] << 16);
+        } else if constexpr (sizeof(T) == 2) {
+            const auto h = __builtin_bit_cast(Pair<T>, c.w[k / 2]);
+            out[k] = (float)((k & 1) ? h.hi : h.lo);
+        } else if constexpr (sizeof(T) == 4) {
+            out[k] = __builtin_bit_cast(T, c.w[k]);
+        } else {
+            out[k] = __builtin_bit_cast(T, (uint64_t)c.w[2 * k + 1] << 32 | c.w[2 * k]);
+        }
+    }
+}
+template <class T>
+__device__ inline void narrow_chunk(const wide_t<T> (&in)[kChunk], Raw<T>& c) {
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) {
+        if constexpr (sizeof(T) == 2) {
+            if (k & 1) c.w[k / 2] = __builtin_bit_cast(uint32_t, Pair<T>{(T)in[k - 1], (T)in[k]});
+        } else if constexpr (sizeof(T) == 4) {
+            c.w[k] = __builtin_bit_cast(uint32_t, in[k]);
+        } else {
+            const uint64_t b = __builtin_bit_cast(uint64_t, in[k]);
+            c.w[2 * k] = (uint32_t)b; c.w[2 * k + 1] = (uint32_t)(b >> 32);
+        }
+    }
+}
+template <class T>
+__device__ inline void load_chunk(const T* p, int count, wide_t<T> (&out)[kChunk]) {
+    Raw<T> c;
+    fetch_chunk(p, count, c);
+    widen_chunk(c, out);
+}
+template <class T>
+__device__ inline void store_chunk(T* p, int count, const wide_t<T> (&in)[kChunk]) {
+    Raw<T> c;
+    narrow_chunk<T>(in, c);
+    put_chunk(p, count, c);
+}
+// Keeps the compiler from holding on to what it formed of the words before.
+template <class T>
+__device__ inline void forget(Raw<T>& c) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords; ++i) asm volatile("" : "+v"(c.w[i]));
+}
+// How many of the eight columns from `col` on exist.
+template <class I>
+__device__ inline int chunk_count(I cols, I col) {
+    const I room = cols - col;
+    return room < 0 ? 0 : room < kChunk ? (int)room : kChunk;
+}
+// Values behind a row's end become zero.
+template <class A>
+__device__ inline void clear_tail(int count, A (&v)[kChunk]) {
+    if (count < kChunk) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) v[k] = k < count ? v[k] : (A)0;
     }
 }
 
@@ -83,42 +203,96 @@ __device__ inline void drop_offset(const DropArgs& d, uint32_t (&off)[2]) {
     off[0] = (uint32_t)o; off[1] = (uint32_t)(o >> 32);
 }
 
-// A dropped value becomes zero whatever it was: infinities and NaN do not pass through the product.
-template <class A>
-__device__ inline void drop_chunk(const DropArgs& d, A scale, const uint32_t (&w)[4], A (&v)[kChunk]) {
+// A bit for each of the eight units: set where it is kept.
+__device__ inline uint32_t keep_bits(const DropArgs& d, const uint32_t (&off)[2], uint32_t chunk, uint32_t row) {
+    uint32_t w[4], bits = 0;
+    draw_words(d, off, chunk, row, w);
 #pragma unroll
     for (int k = 0; k < kChunk; ++k) {
         const uint32_t draw = (k & 1) ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu;
-        v[k] = draw >= d.threshold ? v[k] * scale : (A)0;
+        bits |= draw >= d.threshold ? 1u << k : 0u;
     }
+    return bits;
+}
+// A dropped value becomes zero whatever it was: infinities and NaN do not pass through the product.
+template <class A>
+__device__ inline void drop_chunk(uint32_t bits, A scale, A (&v)[kChunk]) {
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) v[k] = (bits >> k & 1) ? v[k] * scale : (A)0;
 }
 
 // ---- sums over the threads of a row ---------------------------------------------------------------
+// One step of a sum over 2 * D lanes whose halves hold a value each: every lane adds the other half's value.  Steps
+// within 16 lanes are data-parallel moves of the vector unit, the two beyond swap rows of 16 or 32 lanes; nothing goes
+// through LDS.
+template <int D>
+__device__ inline uint32_t other_half(uint32_t v) {
+    if constexpr (D == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, true);        // lanes 1 0 3 2
+    else if constexpr (D == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, true);   // lanes 2 3 0 1
+    else if constexpr (D == 4) return __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);  // 8 lanes mirrored
+    else return __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true);                        // 16 lanes mirrored
+}
+template <int D>
+__device__ inline void halves(uint32_t v, uint32_t& lo, uint32_t& hi) {
+    if constexpr (D == 16) {
+        const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        lo = p[0]; hi = p[1];
+    } else {
+        const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        lo = p[0]; hi = p[1];
+    }
+}
+template <int D>
+__device__ inline float add_half(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    if constexpr (D < 16) return v + __builtin_bit_cast(float, other_half<D>(b));
+    uint32_t lo, hi;
+    halves<D < 16 ? 16 : D>(b, lo, hi);
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+template <int D>
+__device__ inline double add_half(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    if constexpr (D < 16) {
+        const uint64_t o = (uint64_t)other_half<D>((uint32_t)(b >> 32)) << 32 | other_half<D>((uint32_t)b);
+        return v + __builtin_bit_cast(double, o);
+    }
+    uint32_t l0, l1, h0, h1;
+    halves<D < 16 ? 16 : D>((uint32_t)b, l0, h0);
+    halves<D < 16 ? 16 : D>((uint32_t)(b >> 32), l1, h1);
+    return __builtin_bit_cast(double, (uint64_t)l1 << 32 | l0) + __builtin_bit_cast(double, (uint64_t)h1 << 32 | h0);
+}
+// Sum over N consecutive lanes, N a power of two; every lane gets it.
+template <int N, class A>
+__device__ inline A lane_sum(A v) {
+    if constexpr (N > 1) v = add_half<1>(v);
+    if constexpr (N > 2) v = add_half<2>(v);
+    if constexpr (N > 4) v = add_half<4>(v);
+    if constexpr (N > 8) v = add_half<8>(v);
+    if constexpr (N > 16) v = add_half<16>(v);
+    if constexpr (N > 32) v = add_half<32>(v);
+    return v;
+}
+
 // N sums at once over TPR consecutive lanes (TPR <= 64) or over the whole workgroup of TPR threads, in a fixed order;
-// every thread gets them.  The workgroup form alternates between two LDS buffers, so one barrier per call is enough:
-// a buffer is written again only after the barrier of the call between.
-template <class A, int TPR, int N>
+// every thread gets them.  The workgroup form alternates between two LDS buffers, so one barrier a call is enough: a
+// buffer is written again only after the barrier of the call between.
+template <int TPR, int N> constexpr int kRowLds = TPR > 64 ? 2 * (TPR / 64) * N : 1;
+template <int TPR, int N, class A>
 __device__ inline void row_sums(A (&v)[N], A* lds, int& flip) {
 #pragma unroll
-    for (int m = (TPR < 64 ? TPR : 64) / 2; m > 0; m >>= 1) {
-#pragma unroll
-        for (int n = 0; n < N; ++n) v[n] += __shfl_xor(v[n], m, 64);
-    }
+    for (int n = 0; n < N; ++n) v[n] = lane_sum<(TPR < 64 ? TPR : 64)>(v[n]);
     if constexpr (TPR > 64) {
         constexpr int kWaves = TPR / 64;
         A* buf = lds + (flip & 1) * kWaves * 2;
         ++flip;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) buf[(threadIdx.x >> 6) * 2 + n] = v[n];
+            for (int n = 0; n < N; ++n) buf[n * kWaves + (threadIdx.x >> 6)] = v[n];
         }
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            A s = buf[n];
-            for (int w = 1; w < kWaves; ++w) s += buf[w * 2 + n];
-            v[n] = s;
-        }
+        for (int n = 0; n < N; ++n) v[n] = lane_sum<kWaves>(buf[n * kWaves + threadIdx.x % kWaves]);
     }
 }
 
@@ -164,14 +338,99 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T
     if (g >= s.chunks) return;
     const uint32_t r = (uint32_t)(((uint64_t)g * s.magic) >> s.shift), c = g - r * s.per_row;
     const int64_t row = s.row0 + r, col = (int64_t)c * kChunk;
-    const int count = (int)(s.cols - col < kChunk ? s.cols - col : kChunk);
-    wide_t<T> v[kChunk];
-    load_chunk(x + row * s.x_stride + col, count, v);
-    uint32_t off[2], w[4];
+    const int count = chunk_count(s.cols, col);
+    Raw<T> raw;
+    fetch_chunk(x + row * s.x_stride + col, count, raw);
+    uint32_t off[2];
     drop_offset(d, off);
-    draw_words(d, off, c, (uint32_t)row, w);
-    drop_chunk(d, (wide_t<T>)d.scale, w, v);
+    const uint32_t bits = keep_bits(d, off, c, (uint32_t)row);
+    wide_t<T> v[kChunk];
+    widen_chunk(raw, v);
+    drop_chunk(bits, (wide_t<T>)d.scale, v);
     store_chunk(y + row * s.y_stride + col, count, v);
+}
+
+// ---- layer norm, forward: rows that fit the registers of their threads ---------------------------------
+// TPR threads hold a row, NV chunks of eight columns each: it is read once, and while it is worked on the next row
+// is on its way.  TPR <= 64: 256 / TPR rows side by side in a workgroup, no barrier; else a row per workgroup.
+constexpr int norm_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+
+template <class T, int TPR, int NV, bool DROP>
+__global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArgs a) {
+    using A = wide_t<T>;
+    constexpr int kRows = norm_threads(TPR) / TPR;
+    constexpr bool kHold = NV == 1 && sizeof(T) < 8;   // registers for the weights
+    __shared__ A lds[kRowLds<TPR, 2>];
+    int flip = 0;
+    const int t = threadIdx.x % TPR, cols = (int)a.cols;
+    int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    const A inv = (A)a.inv_cols, scale = (A)a.drop.scale;
+    const T* weight = static_cast<const T*>(a.weight);
+    const T* bias = static_cast<const T*>(a.bias);
+    uint32_t off[2] = {0, 0};
+    if constexpr (DROP) drop_offset(a.drop, off);
+    Raw<T> raw[NV];
+    auto fetch = [&](int64_t r) {
+        const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int col = (t + v * TPR) * kChunk;
+            fetch_chunk(x + col, chunk_count(cols, col), raw[v]);
+        }
+    };
+    auto gains = [&](int col, A (&g)[kChunk], A (&b)[kChunk]) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) { g[k] = 1; b[k] = 0; }
+        if (weight) load_chunk(weight + col, chunk_count(cols, col), g);
+        if (bias) load_chunk(bias + col, chunk_count(cols, col), b);
+    };
+    if (row < a.rows) fetch(row);
+    A hg[kChunk], hb[kChunk];
+    if constexpr (kHold) gains(t * kChunk, hg, hb);
+    while (row < a.rows) {
+        A h[NV][kChunk];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) widen_chunk(raw[v], h[v]);
+        const int64_t next = row + step;
+        if (next < a.rows) fetch(next);
+        A s[1] = {0};
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if constexpr (DROP) drop_chunk(keep_bits(a.drop, off, (uint32_t)(t + v * TPR), (uint32_t)row), scale, h[v]);
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) s[0] += h[v][k];   // zero behind the row's end
+        }
+        row_sums<TPR>(s, lds, flip);
+        const A m = s[0] * inv;
+        A q[2] = {0, 0};
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) h[v][k] -= m;
+            clear_tail(chunk_count(cols, (t + v * TPR) * kChunk), h[v]);
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) { q[0] += h[v][k]; q[1] += h[v][k] * h[v][k]; }
+        }
+        row_sums<TPR>(q, lds, flip);
+        const A d = q[0] * inv;
+        A var = q[1] * inv - d * d;
+        var = var < 0 ? (A)0 : var;   // keeps NaN
+        const A r = inverse_root(var + (A)a.eps);
+        if (t == 0 && a.mean) { static_cast<A*>(a.mean)[row] = m + d; static_cast<A*>(a.rstd)[row] = r; }
+        T* y = static_cast<T*>(a.y) + row * a.y_stride;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int col = (t + v * TPR) * kChunk;
+            if (col >= cols) continue;
+            A g[kChunk], b[kChunk];
+            if constexpr (!kHold) gains(col, g, b);
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) h[v][k] = (h[v][k] - d) * r * (kHold ? hg[k] : g[k]) + (kHold ? hb[k] : b[k]);
+            store_chunk(y + col, chunk_count(cols, col), h[v]);
+        }
+        row = next;
+    }
 }
 
 // ---- layer norm, forward: any width ------------------------------------------------------------------
@@ -187,36 +446,32 @@ __device__ inline void norm_forward_row(const NormArgs& a, int64_t row, wide_t<T
     if (DROP && !(SETS && a.sets.set_ctr)) drop_offset(a.drop, pl.off);
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     T* y = static_cast<T*>(a.y) + row * a.y_stride;
-    const A inv = (A)(1.0 / (double)a.cols), scale = (A)a.drop.scale;
+    const A inv = (A)a.inv_cols, scale = (A)a.drop.scale;
     auto load = [&](int64_t col, int& count, A (&h)[kChunk]) {
-        count = (int)(a.cols - col < kChunk ? a.cols - col : kChunk);
+        count = chunk_count(a.cols, col);
         load_chunk(x + col, count, h);
-        if constexpr (DROP) {
-            uint32_t w[4];
-            draw_words(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row, w);
-            drop_chunk(a.drop, scale, w, h);
-        }
+        if constexpr (DROP) drop_chunk(keep_bits(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row), scale, h);
     };
     A s[1] = {0};
     for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
         A h[kChunk]; int count;
         load(col, count, h);
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) s[0] += k < count ? h[k] : (A)0;
+        for (int k = 0; k < kChunk; ++k) s[0] += h[k];
     }
-    row_sums<A, TPR, 1>(s, lds, flip);
+    row_sums<TPR>(s, lds, flip);
     const A m = s[0] * inv;
     A q[2] = {0, 0};
     for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
         A h[kChunk]; int count;
         load(col, count, h);
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) {
-            const A c = k < count ? h[k] - m : (A)0;
-            q[0] += c; q[1] += c * c;
-        }
+        for (int k = 0; k < kChunk; ++k) h[k] -= m;
+        clear_tail(count, h);
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) { q[0] += h[k]; q[1] += h[k] * h[k]; }
     }
-    row_sums<A, TPR, 2>(q, lds, flip);
+    row_sums<TPR>(q, lds, flip);
     const A d = q[0] * inv;
     A var = q[1] * inv - d * d;
     var = var < 0 ? (A)0 : var;   // keeps NaN
@@ -243,7 +498,7 @@ constexpr int64_t kMaxBlocks = (int64_t)1 << 20;
 
 template <class T, int TPR, bool DROP, bool SETS>
 __global__ __launch_bounds__(256) void norm_forward_walk_kernel(NormArgs a) {
-    __shared__ wide_t<T> lds[TPR > 64 ? 2 * (TPR / 64) * 2 : 1];
+    __shared__ wide_t<T> lds[kRowLds<TPR, 2>];
     int flip = 0;
     constexpr int kRows = 256 / TPR;
     for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; row < a.rows; row += (int64_t)gridDim.x * kRows)
@@ -271,8 +526,7 @@ __device__ inline void column_sums(const NormArgs& a, const SplitShape& sh, int6
     if constexpr (SETS) last = first + a.sets.set_used[seg] < last ? first + a.sets.set_used[seg] : last;
     const int lane = threadIdx.x % 4, slot = threadIdx.x / 4;
     const int64_t col = tile * kTileCols + lane * kChunk;
-    const int64_t room = a.cols - col;
-    const int count = (int)(room < 0 ? 0 : room < kChunk ? room : kChunk);
+    const int count = chunk_count(a.cols, col);
     uint32_t off[2] = {0, 0};
     if constexpr (DROP) drop_offset(a.drop, off);
     if (SETS && a.sets.set_ctr) { off[0] = a.sets.set_ctr[2 * seg]; off[1] = a.sets.set_ctr[2 * seg + 1]; }
@@ -286,11 +540,8 @@ __device__ inline void column_sums(const NormArgs& a, const SplitShape& sh, int6
             load_chunk(static_cast<const T*>(a.x) + row * a.x_stride + col, count, h);
             load_chunk(static_cast<const T*>(a.dy) + row * a.dy_stride + col, count, dy);
             const A m = static_cast<const A*>(a.mean)[row], r = static_cast<const A*>(a.rstd)[row];
-            if constexpr (DROP) {
-                uint32_t w[4];
-                draw_words(a.drop, off, (uint32_t)(col / kChunk), (uint32_t)(SETS ? row - first : row), w);
-                drop_chunk(a.drop, scale, w, h);
-            }
+            if constexpr (DROP)
+                drop_chunk(keep_bits(a.drop, off, (uint32_t)(col / kChunk), (uint32_t)(SETS ? row - first : row)), scale, h);
 #pragma unroll
             for (int k = 0; k < kChunk; ++k) {
                 gw[k] += dy[k] * ((h[k] - m) * r);
@@ -334,15 +585,15 @@ __device__ inline void norm_backward_row(const NormArgs& a, int64_t row, wide_t<
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
     T* dx = static_cast<T*>(a.dx) + row * a.y_stride;
     const T* weight = a.weight ? static_cast<const T*>(a.weight) + pl.weight : nullptr;
-    const A inv = (A)(1.0 / (double)a.cols), scale = (A)a.drop.scale;
+    const A inv = (A)a.inv_cols, scale = (A)a.drop.scale;
     const A m = static_cast<const A*>(a.mean)[row], r = static_cast<const A*>(a.rstd)[row];
-    auto load = [&](int64_t col, int& count, A (&u)[kChunk], A (&g)[kChunk], uint32_t (&w)[4]) {
-        count = (int)(a.cols - col < kChunk ? a.cols - col : kChunk);
+    auto load = [&](int64_t col, int& count, A (&u)[kChunk], A (&g)[kChunk], uint32_t& bits) {
+        count = chunk_count(a.cols, col);
         load_chunk(x + col, count, u);
         load_chunk(dy + col, count, g);
         if constexpr (DROP) {
-            draw_words(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row, w);
-            drop_chunk(a.drop, scale, w, u);
+            bits = keep_bits(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row);
+            drop_chunk(bits, scale, u);
         }
         A gain[kChunk];
         if (weight) load_chunk(weight + col, count, gain);
@@ -354,22 +605,20 @@ __device__ inline void norm_backward_row(const NormArgs& a, int64_t row, wide_t<
     };
     A s[2] = {0, 0};
     for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
-        A u[kChunk], g[kChunk]; uint32_t w[4]; int count;
-        load(col, count, u, g, w);
+        A u[kChunk], g[kChunk]; uint32_t bits = 0; int count;
+        load(col, count, u, g, bits);
+        clear_tail(count, u);   // g is zero there, but 0 * u need not be
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) {
-            s[0] += k < count ? g[k] : (A)0;
-            s[1] += k < count ? g[k] * u[k] : (A)0;
-        }
+        for (int k = 0; k < kChunk; ++k) { s[0] += g[k]; s[1] += g[k] * u[k]; }
     }
-    row_sums<A, TPR, 2>(s, lds, flip);
+    row_sums<TPR>(s, lds, flip);
     const A c1 = s[0] * inv, c2 = s[1] * inv;
     for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
-        A u[kChunk], g[kChunk]; uint32_t w[4]; int count;
-        load(col, count, u, g, w);
+        A u[kChunk], g[kChunk]; uint32_t bits = 0; int count;
+        load(col, count, u, g, bits);
 #pragma unroll
         for (int k = 0; k < kChunk; ++k) g[k] = ((g[k] - c1) - u[k] * c2) * r;
-        if constexpr (DROP) drop_chunk(a.drop, scale, w, g);
+        if constexpr (DROP) drop_chunk(bits, scale, g);
         store_chunk(dx + col, count, g);
     }
 }
@@ -388,6 +637,147 @@ __global__ __launch_bounds__(256) void norm_backward_split_kernel(NormArgs a, Sp
         for (int64_t b = (int64_t)blockIdx.x - sh.row_blocks; b < sh.col_tiles * sh.segs; b += stride) {
             column_sums<T, DROP, SETS>(a, sh, b, lds);
             __syncthreads();   // the sums are read before the next tile's are written
+        }
+    }
+}
+
+// ---- layer norm, backward: rows that fit the registers of their threads ---------------------------------
+// One pass over x and dy writes dx and keeps sums of dy u and dy for the thread's columns over all rows of its
+// workgroup, in registers; at the end the workgroup's rows are summed (lanes, then waves, in a fixed order) and
+// one partial row of both gradients is left in the workspace for norm_reduce_kernel.  x and dy stay as they were
+// loaded: u and g are formed twice, before and after the row's two means, which is cheaper than the registers of a
+// widened copy.
+template <class T, int TPR, int NV, bool DROP>
+__global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormArgs a) {
+    using A = wide_t<T>;
+    constexpr int kRows = norm_threads(TPR) / TPR;
+    constexpr bool kAhead = NV * sizeof(T) <= 4;     // registers for the next row
+    constexpr bool kHold = NV == 1 && sizeof(T) < 8; // registers for the weights
+    constexpr int kCols = TPR * NV * kChunk;
+    __shared__ A lds[TPR > 64 ? kRowLds<TPR, 2> : 4 * kCols];
+    int flip = 0;
+    const int t = threadIdx.x % TPR, cols = (int)a.cols;
+    int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    const T* weight = static_cast<const T*>(a.weight);
+    const A inv = (A)a.inv_cols, scale = (A)a.drop.scale;
+    uint32_t off[2] = {0, 0};
+    if constexpr (DROP) drop_offset(a.drop, off);
+    A gw[NV][kChunk], gb[NV][kChunk], hg[kChunk];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) gw[v][k] = gb[v][k] = 0;
+    auto gains = [&](int v, A (&g)[kChunk]) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) g[k] = 1;
+        const int col = (t + v * TPR) * kChunk;
+        if (weight) load_chunk(weight + col, chunk_count(cols, col), g);
+    };
+    Raw<T> rx[NV], rd[NV], nx[kAhead ? NV : 1], nd[kAhead ? NV : 1];
+    A m = 0, r = 0, nm = 0, nr = 0;
+    auto fetch = [&](int64_t at, Raw<T>* fx, Raw<T>* fd, A& fm, A& fr) {
+        const T* x = static_cast<const T*>(a.x) + at * a.x_stride;
+        const T* dy = static_cast<const T*>(a.dy) + at * a.dy_stride;
+        fm = static_cast<const A*>(a.mean)[at]; fr = static_cast<const A*>(a.rstd)[at];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int col = (t + v * TPR) * kChunk;
+            fetch_chunk(x + col, chunk_count(cols, col), fx[v]);
+            fetch_chunk(dy + col, chunk_count(cols, col), fd[v]);
+        }
+    };
+    if (row < a.rows) fetch(row, rx, rd, m, r);
+    if constexpr (kHold) gains(0, hg);
+    while (row < a.rows) {
+        const int64_t next = row + step;
+        if constexpr (kAhead) {
+            if (next < a.rows) fetch(next, nx, nd, nm, nr);
+        }
+        uint32_t bits[NV];
+        A s[2] = {0, 0};
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            A u[kChunk], g[kChunk], w[kChunk];
+            widen_chunk(rx[v], u);
+            widen_chunk(rd[v], g);
+            if constexpr (!kHold) gains(v, w);
+            if constexpr (DROP) {
+                bits[v] = keep_bits(a.drop, off, (uint32_t)(t + v * TPR), (uint32_t)row);
+                drop_chunk(bits[v], scale, u);
+            }
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) u[k] = (u[k] - m) * r;
+            clear_tail(chunk_count(cols, (t + v * TPR) * kChunk), u);   // g is zero there, but 0 * u need not be
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) {
+                gw[v][k] += g[k] * u[k];
+                gb[v][k] += g[k];
+                g[k] *= kHold ? hg[k] : w[k];
+                s[0] += g[k];
+                s[1] += g[k] * u[k];
+            }
+        }
+        row_sums<TPR>(s, lds, flip);
+        const A c1 = s[0] * inv, c2 = s[1] * inv;
+        if (a.dx) {
+            T* dx = static_cast<T*>(a.dx) + row * a.y_stride;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int col = (t + v * TPR) * kChunk;
+                if (col >= cols) continue;
+                A u[kChunk], g[kChunk], w[kChunk];
+                forget(rx[v]);
+                forget(rd[v]);
+                widen_chunk(rx[v], u);
+                widen_chunk(rd[v], g);
+                if constexpr (!kHold) gains(v, w);
+                if constexpr (DROP) drop_chunk(bits[v], scale, u);
+#pragma unroll
+                for (int k = 0; k < kChunk; ++k) {
+                    u[k] = (u[k] - m) * r;
+                    g[k] *= kHold ? hg[k] : w[k];
+                    g[k] = ((g[k] - c1) - u[k] * c2) * r;
+                }
+                if constexpr (DROP) drop_chunk(bits[v], scale, g);
+                store_chunk(dx + col, chunk_count(cols, col), g);
+            }
+        }
+        row = next;
+        if constexpr (kAhead) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) { rx[v] = nx[v]; rd[v] = nd[v]; }
+            m = nm; r = nr;
+        } else {
+            if (row < a.rows) fetch(row, rx, rd, m, r);
+        }
+    }
+    if (!a.workspace) return;
+    A* part = static_cast<A*>(a.workspace) + (int64_t)blockIdx.x * 2 * cols;
+    if constexpr (TPR > 64) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) {
+                const int col = (t + v * TPR) * kChunk + k;
+                if (col < cols) { part[col] = gw[v][k]; part[cols + col] = gb[v][k]; }
+            }
+    } else {
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int k = 0; k < kChunk; ++k) {
+                    A z = which ? gb[v][k] : gw[v][k];
+#pragma unroll
+                    for (int n = TPR; n < 64; n <<= 1) z += __shfl_xor(z, n, 64);
+                    if ((threadIdx.x & 63) < TPR) lds[(threadIdx.x >> 6) * kCols + (t + v * TPR) * kChunk + k] = z;
+                }
+            __syncthreads();
+            for (int c = threadIdx.x; c < cols; c += 256)
+                part[which * cols + c] = (lds[c] + lds[kCols + c]) + (lds[2 * kCols + c] + lds[3 * kCols + c]);
         }
     }
 }
@@ -442,6 +832,41 @@ auto with_flag(bool on, F f) {
     return on ? f(std::true_type{}) : f(std::false_type{});
 }
 
+// Threads of a row and chunks of a thread for rows that are held in registers: calls f(threads, chunks) and returns
+// true, or returns false for rows that are too wide.
+template <int N> using int_c = std::integral_constant<int, N>;
+template <class T, bool FORWARD, class F>
+bool with_row_shape(int64_t cols, F f) {
+    if (cols <= 32) f(int_c<4>{}, int_c<1>{});
+    else if (cols <= 64) f(int_c<8>{}, int_c<1>{});
+    else if (cols <= 128) f(int_c<16>{}, int_c<1>{});
+    else if (cols <= 256) f(int_c<32>{}, int_c<1>{});
+    else if (cols <= 512) f(int_c<64>{}, int_c<1>{});
+    else if (cols <= 1024) f(int_c<64>{}, int_c<2>{});
+    else if (cols <= 2048) f(int_c<256>{}, int_c<1>{});
+    else if (cols <= 4096) f(int_c<256>{}, int_c<2>{});
+    else if (cols <= 8192) f(int_c<512>{}, int_c<2>{});
+    else if constexpr (sizeof(T) < 8) {
+        if (cols <= 16384) f(int_c<512>{}, int_c<4>{});
+        else if (cols <= 24576) f(int_c<512>{}, int_c<6>{});
+        else return false;
+    } else return false;
+    return true;
+}
+
+#ifndef FWD_T
+#define FWD_T 2048*256
+#define BWD_T 1024*256
+#endif
+constexpr int64_t kForwardThreads = FWD_T, kBackwardThreads = BWD_T;
+constexpr int64_t kSplitRows = 1024;
+
+template <int TPR>
+int64_t backward_blocks(int64_t rows) {
+    constexpr int kRows = norm_threads(TPR) / TPR;
+    return std::min((rows + kRows - 1) / kRows, kBackwardThreads / norm_threads(TPR));
+}
+
 // Rows of one column workgroup: as many as keep its walk short; more rows than that become segments.
 constexpr int64_t kSegRows = 1024;
 
@@ -494,15 +919,20 @@ hipError_t launch_dropout(LayerType type, int64_t rows, int64_t cols, int64_t x_
     return hipGetLastError();
 }
 
-hipError_t launch_norm_forward(LayerType type, const NormArgs& a, hipStream_t s) {
-    if (a.rows == 0) return hipSuccess;
+hipError_t launch_norm_forward(LayerType type, const NormArgs& args, hipStream_t s) {
+    if (args.rows == 0) return hipSuccess;
+    NormArgs a = args;
+    a.inv_cols = 1.0 / (double)a.cols;
     with_type(type, [&](auto t) {
         using T = decltype(t);
         with_flag(a.drop.threshold != 0, [&](auto drop) {
             constexpr bool D = decltype(drop)::value;
-            if (a.cols <= 2048)
-                hipLaunchKernelGGL((norm_forward_walk_kernel<T, 64, D, false>), dim3((unsigned)std::min((a.rows + 3) / 4, kMaxBlocks)), dim3(256), 0, s, a);
-            else
+            const bool held = with_row_shape<T, true>(a.cols, [&](auto tpr, auto nv) {
+                constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, kRows = norm_threads(TPR) / TPR;
+                const int64_t blocks = std::min((a.rows + kRows - 1) / kRows, kForwardThreads / norm_threads(TPR));
+                hipLaunchKernelGGL((norm_forward_kernel<T, TPR, NV, D>), dim3((unsigned)blocks), dim3(norm_threads(TPR)), 0, s, a);
+            });
+            if (!held)
                 hipLaunchKernelGGL((norm_forward_walk_kernel<T, 256, D, false>), dim3((unsigned)std::min(a.rows, kMaxBlocks)), dim3(256), 0, s, a);
         });
     });
@@ -510,32 +940,55 @@ hipError_t launch_norm_forward(LayerType type, const NormArgs& a, hipStream_t s)
 }
 
 size_t norm_backward_workspace(LayerType type, int64_t rows, int64_t cols) {
-    const int64_t segs = (rows + kSegRows - 1) / kSegRows;
-    return segs > 1 ? (size_t)segs * 2 * cols * (type == kF64 ? 8 : 4) : 0;
+    return with_type(type, [&](auto t) -> size_t {
+        using T = decltype(t);
+        int64_t parts = 0;
+        if (rows > kSplitRows)
+            with_row_shape<T, false>(cols, [&](auto tpr, auto) { parts = backward_blocks<decltype(tpr)::value>(rows); });
+        if (!parts) {
+            const int64_t segs = (rows + kSegRows - 1) / kSegRows;
+            parts = segs > 1 ? segs : 0;
+        }
+        return (size_t)parts * 2 * cols * sizeof(wide_t<T>);
+    });
 }
 
-hipError_t launch_norm_backward(LayerType type, const NormArgs& a, hipStream_t s) {
+hipError_t launch_norm_backward(LayerType type, const NormArgs& args, hipStream_t s) {
+    NormArgs a = args;
+    a.inv_cols = 1.0 / (double)a.cols;
     with_type(type, [&](auto t) {
         using T = decltype(t);
+        const bool vectors = a.dweight || a.dbias;
         if (a.rows == 0) {
-            if (a.dweight || a.dbias)
+            if (vectors)
                 hipLaunchKernelGGL(norm_zero_kernel<T>, dim3((unsigned)((a.cols + 255) / 256)), dim3(256), 0, s,
                                    static_cast<T*>(a.dweight), static_cast<T*>(a.dbias), a.cols);
             return;
         }
-        const bool wide = a.cols > 2048;
-        SplitShape sh = split_shape(a, wide ? 256 : 64);
-        const int64_t col_blocks = a.dweight || a.dbias ? std::min(sh.col_tiles * sh.segs, kMaxBlocks) : 0;
-        if (sh.row_blocks + col_blocks == 0) return;
-        const dim3 grid((unsigned)(sh.row_blocks + col_blocks));
+        if (!vectors && !a.dx) return;
+        int64_t parts = 0;
         with_flag(a.drop.threshold != 0, [&](auto drop) {
             constexpr bool D = decltype(drop)::value;
+            if (a.rows > kSplitRows)
+                with_row_shape<T, false>(a.cols, [&](auto tpr, auto nv) {
+                    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+                    NormArgs b = a;
+                    if (!vectors) b.workspace = nullptr;
+                    parts = backward_blocks<TPR>(a.rows);
+                    hipLaunchKernelGGL((norm_backward_kernel<T, TPR, NV, D>), dim3((unsigned)parts), dim3(norm_threads(TPR)), 0, s, b);
+                });
+            if (parts) return;
+            const bool wide = a.cols > 2048;
+            const SplitShape sh = split_shape(a, wide ? 256 : 64);
+            const int64_t col_blocks = vectors ? std::min(sh.col_tiles * sh.segs, kMaxBlocks) : 0;
+            const dim3 grid((unsigned)(sh.row_blocks + col_blocks));
             if (wide) hipLaunchKernelGGL((norm_backward_split_kernel<T, 256, D, false>), grid, dim3(256), 0, s, a, sh);
             else hipLaunchKernelGGL((norm_backward_split_kernel<T, 64, D, false>), grid, dim3(256), 0, s, a, sh);
+            if (sh.segs > 1) parts = sh.segs;
         });
-        if (col_blocks && sh.segs > 1)
+        if (parts && vectors)
             hipLaunchKernelGGL(norm_reduce_kernel<T>, dim3((unsigned)((2 * a.cols + 15) / 16)), dim3(1024), 0, s,
-                               static_cast<const wide_t<T>*>(a.workspace), sh.segs, a.cols, static_cast<T*>(a.dweight),
+                               static_cast<const wide_t<T>*>(a.workspace), parts, a.cols, static_cast<T*>(a.dweight),
                                static_cast<T*>(a.dbias));
     });
     return hipGetLastError();

@@ -39,6 +39,7 @@ struct NormArgs {
     void *dweight, *dbias;       // [cols], or [sets][cols] with sets
     void* workspace;
     double eps;
+    double inv_cols;             // 1 / cols, set by the launchers
     DropArgs drop;
     NormSets sets;               // sets.count == 0: one set of weights
 };
