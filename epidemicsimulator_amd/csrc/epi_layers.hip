@@ -203,22 +203,24 @@ __device__ inline void drop_offset(const DropArgs& d, uint32_t (&off)[2]) {
     off[0] = (uint32_t)o; off[1] = (uint32_t)(o >> 32);
 }
 
-// A bit for each of the eight units: set where it is kept.
-__device__ inline uint32_t keep_bits(const DropArgs& d, const uint32_t (&off)[2], uint32_t chunk, uint32_t row) {
-    uint32_t w[4], bits = 0;
-    draw_words(d, off, chunk, row, w);
-#pragma unroll
-    for (int k = 0; k < kChunk; ++k) {
-        const uint32_t draw = (k & 1) ? w[k >> 1] >> 16 : w[k >> 1] & 0xffffu;
-        bits |= draw >= d.threshold ? 1u << k : 0u;
-    }
-    return bits;
+// Which of the eight units are kept: the draw of 16 bits in the upper half of a word w is at least the threshold t
+// exactly where w > t * 2^16 - 1, whatever the lower half holds; the draw in the lower half is shifted there.  For
+// t = 2^16 nothing is above the border; t = 0 has none, and is not asked for.
+struct Keep {
+    uint32_t w[4], border;
+    __device__ bool operator()(int k) const { return ((k & 1) ? w[k >> 1] : w[k >> 1] << 16) > border; }
+};
+__device__ inline Keep keep_of(const DropArgs& d, const uint32_t (&off)[2], uint32_t chunk, uint32_t row) {
+    Keep keep;
+    draw_words(d, off, chunk, row, keep.w);
+    keep.border = (uint32_t)(((uint64_t)d.threshold << 16) - 1);
+    return keep;
 }
 // A dropped value becomes zero whatever it was: infinities and NaN do not pass through the product.
 template <class A>
-__device__ inline void drop_chunk(uint32_t bits, A scale, A (&v)[kChunk]) {
+__device__ inline void drop_chunk(const Keep& keep, A scale, A (&v)[kChunk]) {
 #pragma unroll
-    for (int k = 0; k < kChunk; ++k) v[k] = (bits >> k & 1) ? v[k] * scale : (A)0;
+    for (int k = 0; k < kChunk; ++k) v[k] = keep(k) ? v[k] * scale : (A)0;
 }
 
 // ---- sums over the threads of a row ---------------------------------------------------------------
@@ -332,7 +334,7 @@ struct DropShape {
     int64_t cols, x_stride, y_stride;
 };
 
-template <class T>
+template <class T, bool DROP>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, DropShape s, DropArgs d) {
     const uint32_t g = blockIdx.x * 256u + threadIdx.x;
     if (g >= s.chunks) return;
@@ -341,19 +343,73 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T
     const int count = chunk_count(s.cols, col);
     Raw<T> raw;
     fetch_chunk(x + row * s.x_stride + col, count, raw);
-    uint32_t off[2];
-    drop_offset(d, off);
-    const uint32_t bits = keep_bits(d, off, c, (uint32_t)row);
     wide_t<T> v[kChunk];
     widen_chunk(raw, v);
-    drop_chunk(bits, (wide_t<T>)d.scale, v);
+    if constexpr (DROP) {
+        uint32_t off[2];
+        drop_offset(d, off);
+        drop_chunk(keep_of(d, off, c, (uint32_t)row), (wide_t<T>)d.scale, v);
+    }
     store_chunk(y + row * s.y_stride + col, count, v);
 }
 
 // ---- layer norm, forward: rows that fit the registers of their threads ---------------------------------
 // TPR threads hold a row, NV chunks of eight columns each: it is read once, and while it is worked on the next row
 // is on its way.  TPR <= 64: 256 / TPR rows side by side in a workgroup, no barrier; else a row per workgroup.
-constexpr int norm_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+constexpr int norm_threads(int tpr) { return tpr > 64 ? tpr : 256; }
+
+// The chunk of a row of at least eight columns that a thread works on.  Where the row's end cuts it, it is moved back
+// to the last eight columns, and its first `skip` columns are another thread's too: both form the same values for
+// them from the same inputs and both store them, but only the other counts them in sums.  So no access and no value
+// needs a case of its own.  skip = 8: no column of the row is left for this thread, which loads but stores nothing.
+struct Spot {
+    int col, skip;
+};
+__device__ inline Spot spot_of(int cols, int chunk) {
+    const int col = chunk * kChunk, at = min(col, cols - kChunk);
+    return {at, min(col - at, kChunk)};
+}
+template <class A>
+__device__ inline void clear_head(int skip, A (&v)[kChunk]) {
+    if (skip > 0) {
+#pragma unroll
+        for (int k = 0; k < kChunk; ++k) v[k] = k < skip ? (A)0 : v[k];
+    }
+}
+// keep_of for a spot: one that was moved back takes its draws from two counters.
+__device__ inline Keep keep_at(const DropArgs& d, const uint32_t (&off)[2], const Spot& p, uint32_t row) {
+    const uint32_t chunk = (uint32_t)p.col / kChunk, shift = (uint32_t)p.col % kChunk;
+    Keep keep = keep_of(d, off, chunk, row);
+    if (shift) {
+        uint32_t w[8];
+        const Keep next = keep_of(d, off, chunk + 1, row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { w[i] = keep.w[i]; w[i + 4] = next.w[i]; }
+        if (shift & 4) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+        }
+        if (shift & 2) {
+#pragma unroll
+            for (int i = 0; i < 7; ++i) w[i] = w[i + 1];
+        }
+        if (shift & 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = w[i] >> 16 | w[i + 1] << 16;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) keep.w[i] = w[i];
+    }
+    return keep;
+}
+template <class T>
+__device__ inline void fetch_full(const T* p, Raw<T>& c) { fetch_part<T, kChunk>(p, c.w); }
+template <class T>
+__device__ inline void load_full(const T* p, wide_t<T> (&out)[kChunk]) {
+    Raw<T> c;
+    fetch_full(p, c);
+    widen_chunk(c, out);
+}
 
 template <class T, int TPR, int NV, bool DROP>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArgs a) {
@@ -374,20 +430,17 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArg
     auto fetch = [&](int64_t r) {
         const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int col = (t + v * TPR) * kChunk;
-            fetch_chunk(x + col, chunk_count(cols, col), raw[v]);
-        }
+        for (int v = 0; v < NV; ++v) fetch_full(x + spot_of(cols, t + v * TPR).col, raw[v]);
     };
     auto gains = [&](int col, A (&g)[kChunk], A (&b)[kChunk]) {
 #pragma unroll
         for (int k = 0; k < kChunk; ++k) { g[k] = 1; b[k] = 0; }
-        if (weight) load_chunk(weight + col, chunk_count(cols, col), g);
-        if (bias) load_chunk(bias + col, chunk_count(cols, col), b);
+        if (weight) load_full(weight + col, g);
+        if (bias) load_full(bias + col, b);
     };
     if (row < a.rows) fetch(row);
     A hg[kChunk], hb[kChunk];
-    if constexpr (kHold) gains(t * kChunk, hg, hb);
+    if constexpr (kHold) gains(spot_of(cols, t).col, hg, hb);
     while (row < a.rows) {
         A h[NV][kChunk];
 #pragma unroll
@@ -397,20 +450,26 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArg
         A s[1] = {0};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if constexpr (DROP) drop_chunk(keep_bits(a.drop, off, (uint32_t)(t + v * TPR), (uint32_t)row), scale, h[v]);
+            const Spot p = spot_of(cols, t + v * TPR);
+            if constexpr (DROP) drop_chunk(keep_at(a.drop, off, p, (uint32_t)row), scale, h[v]);
+            A c[kChunk];
 #pragma unroll
-            for (int k = 0; k < kChunk; ++k) s[0] += h[v][k];   // zero behind the row's end
+            for (int k = 0; k < kChunk; ++k) c[k] = h[v][k];
+            clear_head(p.skip, c);
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) s[0] += c[k];
         }
         row_sums<TPR>(s, lds, flip);
         const A m = s[0] * inv;
         A q[2] = {0, 0};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
+            A c[kChunk];
 #pragma unroll
-            for (int k = 0; k < kChunk; ++k) h[v][k] -= m;
-            clear_tail(chunk_count(cols, (t + v * TPR) * kChunk), h[v]);
+            for (int k = 0; k < kChunk; ++k) c[k] = h[v][k] -= m;
+            clear_head(spot_of(cols, t + v * TPR).skip, c);
 #pragma unroll
-            for (int k = 0; k < kChunk; ++k) { q[0] += h[v][k]; q[1] += h[v][k] * h[v][k]; }
+            for (int k = 0; k < kChunk; ++k) { q[0] += c[k]; q[1] += c[k] * c[k]; }
         }
         row_sums<TPR>(q, lds, flip);
         const A d = q[0] * inv;
@@ -421,13 +480,15 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArg
         T* y = static_cast<T*>(a.y) + row * a.y_stride;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int col = (t + v * TPR) * kChunk;
-            if (col >= cols) continue;
+            const Spot p = spot_of(cols, t + v * TPR);
+            if (p.skip == kChunk) continue;
             A g[kChunk], b[kChunk];
-            if constexpr (!kHold) gains(col, g, b);
+            if constexpr (!kHold) gains(p.col, g, b);
 #pragma unroll
             for (int k = 0; k < kChunk; ++k) h[v][k] = (h[v][k] - d) * r * (kHold ? hg[k] : g[k]) + (kHold ? hb[k] : b[k]);
-            store_chunk(y + col, chunk_count(cols, col), h[v]);
+            Raw<T> o;
+            narrow_chunk<T>(h[v], o);
+            put_part<T, kChunk>(y + p.col, o.w);
         }
         row = next;
     }
@@ -450,7 +511,7 @@ __device__ inline void norm_forward_row(const NormArgs& a, int64_t row, wide_t<T
     auto load = [&](int64_t col, int& count, A (&h)[kChunk]) {
         count = chunk_count(a.cols, col);
         load_chunk(x + col, count, h);
-        if constexpr (DROP) drop_chunk(keep_bits(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row), scale, h);
+        if constexpr (DROP) drop_chunk(keep_of(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row), scale, h);
     };
     A s[1] = {0};
     for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
@@ -541,7 +602,7 @@ __device__ inline void column_sums(const NormArgs& a, const SplitShape& sh, int6
             load_chunk(static_cast<const T*>(a.dy) + row * a.dy_stride + col, count, dy);
             const A m = static_cast<const A*>(a.mean)[row], r = static_cast<const A*>(a.rstd)[row];
             if constexpr (DROP)
-                drop_chunk(keep_bits(a.drop, off, (uint32_t)(col / kChunk), (uint32_t)(SETS ? row - first : row)), scale, h);
+                drop_chunk(keep_of(a.drop, off, (uint32_t)(col / kChunk), (uint32_t)(SETS ? row - first : row)), scale, h);
 #pragma unroll
             for (int k = 0; k < kChunk; ++k) {
                 gw[k] += dy[k] * ((h[k] - m) * r);
@@ -587,13 +648,13 @@ __device__ inline void norm_backward_row(const NormArgs& a, int64_t row, wide_t<
     const T* weight = a.weight ? static_cast<const T*>(a.weight) + pl.weight : nullptr;
     const A inv = (A)a.inv_cols, scale = (A)a.drop.scale;
     const A m = static_cast<const A*>(a.mean)[row], r = static_cast<const A*>(a.rstd)[row];
-    auto load = [&](int64_t col, int& count, A (&u)[kChunk], A (&g)[kChunk], uint32_t& bits) {
+    auto load = [&](int64_t col, int& count, A (&u)[kChunk], A (&g)[kChunk], Keep& keep) {
         count = chunk_count(a.cols, col);
         load_chunk(x + col, count, u);
         load_chunk(dy + col, count, g);
         if constexpr (DROP) {
-            bits = keep_bits(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row);
-            drop_chunk(bits, scale, u);
+            keep = keep_of(a.drop, pl.off, (uint32_t)(col / kChunk), pl.row);
+            drop_chunk(keep, scale, u);
         }
         A gain[kChunk];
         if (weight) load_chunk(weight + col, count, gain);
@@ -605,8 +666,8 @@ __device__ inline void norm_backward_row(const NormArgs& a, int64_t row, wide_t<
     };
     A s[2] = {0, 0};
     for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
-        A u[kChunk], g[kChunk]; uint32_t bits = 0; int count;
-        load(col, count, u, g, bits);
+        A u[kChunk], g[kChunk]; Keep keep{}; int count;
+        load(col, count, u, g, keep);
         clear_tail(count, u);   // g is zero there, but 0 * u need not be
 #pragma unroll
         for (int k = 0; k < kChunk; ++k) { s[0] += g[k]; s[1] += g[k] * u[k]; }
@@ -614,11 +675,11 @@ __device__ inline void norm_backward_row(const NormArgs& a, int64_t row, wide_t<
     row_sums<TPR>(s, lds, flip);
     const A c1 = s[0] * inv, c2 = s[1] * inv;
     for (int64_t col = (int64_t)t * kChunk; col < a.cols; col += TPR * kChunk) {
-        A u[kChunk], g[kChunk]; uint32_t bits = 0; int count;
-        load(col, count, u, g, bits);
+        A u[kChunk], g[kChunk]; Keep keep{}; int count;
+        load(col, count, u, g, keep);
 #pragma unroll
         for (int k = 0; k < kChunk; ++k) g[k] = ((g[k] - c1) - u[k] * c2) * r;
-        if constexpr (DROP) drop_chunk(bits, scale, g);
+        if constexpr (DROP) drop_chunk(keep, scale, g);
         store_chunk(dx + col, count, g);
     }
 }
@@ -651,7 +712,8 @@ template <class T, int TPR, int NV, bool DROP>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormArgs a) {
     using A = wide_t<T>;
     constexpr int kRows = norm_threads(TPR) / TPR;
-    constexpr bool kAhead = NV * sizeof(T) <= 4;     // registers for the next row
+    constexpr bool kKeep = NV * sizeof(T) <= 8;      // registers for x and dy of the row
+    constexpr bool kAhead = NV * sizeof(T) <= 4;     // and of the next row
     constexpr bool kHold = NV == 1 && sizeof(T) < 8; // registers for the weights
     constexpr int kCols = TPR * NV * kChunk;
     __shared__ A lds[TPR > 64 ? kRowLds<TPR, 2> : 4 * kCols];
@@ -671,20 +733,20 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
     auto gains = [&](int v, A (&g)[kChunk]) {
 #pragma unroll
         for (int k = 0; k < kChunk; ++k) g[k] = 1;
-        const int col = (t + v * TPR) * kChunk;
-        if (weight) load_chunk(weight + col, chunk_count(cols, col), g);
+        if (weight) load_full(weight + spot_of(cols, t + v * TPR).col, g);
     };
-    Raw<T> rx[NV], rd[NV], nx[kAhead ? NV : 1], nd[kAhead ? NV : 1];
+    Raw<T> rx[kKeep ? NV : 1], rd[kKeep ? NV : 1], nx[kAhead ? NV : 1], nd[kAhead ? NV : 1];
     A m = 0, r = 0, nm = 0, nr = 0;
+    auto fetch_one = [&](int64_t at, int v, Raw<T>& fx, Raw<T>& fd) {
+        const int col = spot_of(cols, t + v * TPR).col;
+        fetch_full(static_cast<const T*>(a.x) + at * a.x_stride + col, fx);
+        fetch_full(static_cast<const T*>(a.dy) + at * a.dy_stride + col, fd);
+    };
     auto fetch = [&](int64_t at, Raw<T>* fx, Raw<T>* fd, A& fm, A& fr) {
-        const T* x = static_cast<const T*>(a.x) + at * a.x_stride;
-        const T* dy = static_cast<const T*>(a.dy) + at * a.dy_stride;
         fm = static_cast<const A*>(a.mean)[at]; fr = static_cast<const A*>(a.rstd)[at];
+        if constexpr (kKeep) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int col = (t + v * TPR) * kChunk;
-            fetch_chunk(x + col, chunk_count(cols, col), fx[v]);
-            fetch_chunk(dy + col, chunk_count(cols, col), fd[v]);
+            for (int v = 0; v < NV; ++v) fetch_one(at, v, fx[v], fd[v]);
         }
     };
     if (row < a.rows) fetch(row, rx, rd, m, r);
@@ -694,23 +756,24 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
         if constexpr (kAhead) {
             if (next < a.rows) fetch(next, nx, nd, nm, nr);
         }
-        uint32_t bits[NV];
+        Keep keep[NV];
         A s[2] = {0, 0};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
+            const Spot p = spot_of(cols, t + v * TPR);
             A u[kChunk], g[kChunk], w[kChunk];
-            widen_chunk(rx[v], u);
-            widen_chunk(rd[v], g);
+            if constexpr (!kKeep) fetch_one(row, v, rx[0], rd[0]);
+            widen_chunk(rx[kKeep ? v : 0], u);
+            widen_chunk(rd[kKeep ? v : 0], g);
             if constexpr (!kHold) gains(v, w);
             if constexpr (DROP) {
-                bits[v] = keep_bits(a.drop, off, (uint32_t)(t + v * TPR), (uint32_t)row);
-                drop_chunk(bits[v], scale, u);
+                keep[v] = keep_at(a.drop, off, p, (uint32_t)row);
+                drop_chunk(keep[v], scale, u);
             }
-#pragma unroll
-            for (int k = 0; k < kChunk; ++k) u[k] = (u[k] - m) * r;
-            clear_tail(chunk_count(cols, (t + v * TPR) * kChunk), u);   // g is zero there, but 0 * u need not be
+            clear_head(p.skip, g);
 #pragma unroll
             for (int k = 0; k < kChunk; ++k) {
+                u[k] = (u[k] - m) * r;
                 gw[v][k] += g[k] * u[k];
                 gb[v][k] += g[k];
                 g[k] *= kHold ? hg[k] : w[k];
@@ -724,23 +787,26 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
             T* dx = static_cast<T*>(a.dx) + row * a.y_stride;
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                const int col = (t + v * TPR) * kChunk;
-                if (col >= cols) continue;
+                const Spot p = spot_of(cols, t + v * TPR);
+                if (p.skip == kChunk) continue;
                 A u[kChunk], g[kChunk], w[kChunk];
-                forget(rx[v]);
-                forget(rd[v]);
-                widen_chunk(rx[v], u);
-                widen_chunk(rd[v], g);
+                if constexpr (!kKeep) fetch_one(row, v, rx[0], rd[0]);
+                forget(rx[kKeep ? v : 0]);
+                forget(rd[kKeep ? v : 0]);
+                widen_chunk(rx[kKeep ? v : 0], u);
+                widen_chunk(rd[kKeep ? v : 0], g);
                 if constexpr (!kHold) gains(v, w);
-                if constexpr (DROP) drop_chunk(bits[v], scale, u);
+                if constexpr (DROP) drop_chunk(keep[v], scale, u);
 #pragma unroll
                 for (int k = 0; k < kChunk; ++k) {
                     u[k] = (u[k] - m) * r;
                     g[k] *= kHold ? hg[k] : w[k];
                     g[k] = ((g[k] - c1) - u[k] * c2) * r;
                 }
-                if constexpr (DROP) drop_chunk(bits[v], scale, g);
-                store_chunk(dx + col, chunk_count(cols, col), g);
+                if constexpr (DROP) drop_chunk(keep[v], scale, g);
+                Raw<T> o;
+                narrow_chunk<T>(g, o);
+                put_part<T, kChunk>(dx + p.col, o.w);
             }
         }
         row = next;
@@ -756,25 +822,27 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
     A* part = static_cast<A*>(a.workspace) + (int64_t)blockIdx.x * 2 * cols;
     if constexpr (TPR > 64) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            const Spot p = spot_of(cols, t + v * TPR);
 #pragma unroll
-            for (int k = 0; k < kChunk; ++k) {
-                const int col = (t + v * TPR) * kChunk + k;
-                if (col < cols) { part[col] = gw[v][k]; part[cols + col] = gb[v][k]; }
-            }
+            for (int k = 0; k < kChunk; ++k)
+                if (k >= p.skip) { part[p.col + k] = gw[v][k]; part[cols + p.col + k] = gb[v][k]; }
+        }
     } else {
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             __syncthreads();
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
+            for (int v = 0; v < NV; ++v) {
+                const Spot p = spot_of(cols, t + v * TPR);
 #pragma unroll
                 for (int k = 0; k < kChunk; ++k) {
                     A z = which ? gb[v][k] : gw[v][k];
 #pragma unroll
                     for (int n = TPR; n < 64; n <<= 1) z += __shfl_xor(z, n, 64);
-                    if ((threadIdx.x & 63) < TPR) lds[(threadIdx.x >> 6) * kCols + (t + v * TPR) * kChunk + k] = z;
+                    if ((threadIdx.x & 63) < TPR && k >= p.skip) lds[(threadIdx.x >> 6) * kCols + p.col + k] = z;
                 }
+            }
             __syncthreads();
             for (int c = threadIdx.x; c < cols; c += 256)
                 part[which * cols + c] = (lds[c] + lds[kCols + c]) + (lds[2 * kCols + c] + lds[3 * kCols + c]);
@@ -833,10 +901,17 @@ auto with_flag(bool on, F f) {
 }
 
 // Threads of a row and chunks of a thread for rows that are held in registers: calls f(threads, chunks) and returns
-// true, or returns false for rows that are too wide.
+// true, or returns false for rows that are too narrow or too wide.  Up to 1,024 columns a row stays in a wave: no
+// barrier.  Beyond, the smallest workgroup with one chunk a thread, while there is one: at 16,384 x 4,096 bfloat16 the
+// backward pass takes 91 us with 512 x 1, 122 with 256 x 2 and 145 with 128 x 4, because the next row's registers
+// then fit beside the sums; the forward pass, which has no sums, does not care (47.2, 50.3, 53.0).  Backward rows that
+// need more registers than a wave has are left to the split kernels, which read x and dy twice: 4,000 x 24,000
+// bfloat16 take 262 us there and 296 with 1,024 x 3, 1,500 x 12,000 double 165 and 299, but 6,000 x 16,000 bfloat16 261
+// and 171 with 1,024 x 2, 3,000 x 8,000 double 237 and 192 with 1,024 x 1.
 template <int N> using int_c = std::integral_constant<int, N>;
 template <class T, bool FORWARD, class F>
 bool with_row_shape(int64_t cols, F f) {
+    if (cols < kChunk) return false;
     if (cols <= 32) f(int_c<4>{}, int_c<1>{});
     else if (cols <= 64) f(int_c<8>{}, int_c<1>{});
     else if (cols <= 128) f(int_c<16>{}, int_c<1>{});
@@ -844,28 +919,39 @@ bool with_row_shape(int64_t cols, F f) {
     else if (cols <= 512) f(int_c<64>{}, int_c<1>{});
     else if (cols <= 1024) f(int_c<64>{}, int_c<2>{});
     else if (cols <= 2048) f(int_c<256>{}, int_c<1>{});
-    else if (cols <= 4096) f(int_c<256>{}, int_c<2>{});
-    else if (cols <= 8192) f(int_c<512>{}, int_c<2>{});
-    else if constexpr (sizeof(T) < 8) {
-        if (cols <= 16384) f(int_c<512>{}, int_c<4>{});
-        else if (cols <= 24576) f(int_c<512>{}, int_c<6>{});
-        else return false;
-    } else return false;
+    else if (cols <= 4096) f(int_c<512>{}, int_c<1>{});
+    else if (cols <= 8192) f(int_c<FORWARD ? 512 : 1024>{}, int_c<FORWARD ? 2 : 1>{});
+    else if constexpr (!FORWARD && sizeof(T) == 8) return false;
+    else if (cols <= 16384) f(int_c<1024>{}, int_c<2>{});
+    else if constexpr (!FORWARD) return false;
+    else if (cols <= 24576) f(int_c<1024>{}, int_c<3>{});
+    else if (cols <= 32768) f(int_c<1024>{}, int_c<4>{});
+    else return false;
     return true;
 }
 
-#ifndef FWD_T
-#define FWD_T 2048*256
-#define BWD_T 1024*256
-#endif
-constexpr int64_t kForwardThreads = FWD_T, kBackwardThreads = BWD_T;
-constexpr int64_t kSplitRows = 1024;
+// Workgroups of the forward pass: several rounds of what the device holds at once, so that a workgroup that falls
+// behind is made up for (819,200 x 128 bfloat16: 80.7 us with 4,096, 76.5 with 8,192 or 16,384, 84.6 with one for
+// every 16 rows, which spends its time on starting them).
+template <int TPR>
+int64_t forward_blocks(int64_t rows) {
+    constexpr int kRows = norm_threads(TPR) / TPR;
+    return std::min((rows + kRows - 1) / kRows, TPR <= 256 ? (int64_t)8192 : (int64_t)2048 * 256 / norm_threads(TPR));
+}
 
+// Workgroups of the backward pass.  Each leaves a partial row of both gradients, so here fewer are better until the
+// device is no longer full: a row in a wave, 512 (24,576 x 128 float: 12.0 us, 13.0 with 256, 14.0 with 1,024), and 768
+// where rows are many (819,200 x 128 bfloat16: 122.8 us, 127.6 with 512, 127.0 with 1,024); a row in a workgroup, what
+// fills the device four waves deep.
 template <int TPR>
 int64_t backward_blocks(int64_t rows) {
     constexpr int kRows = norm_threads(TPR) / TPR;
-    return std::min((rows + kRows - 1) / kRows, kBackwardThreads / norm_threads(TPR));
+    const int64_t most = TPR > 64 ? (int64_t)1024 * 256 / norm_threads(TPR)
+                                  : std::min<int64_t>(768, std::max<int64_t>(rows / (kRows * 16), 512));
+    return std::min((rows + kRows - 1) / kRows, most);
 }
+// Up to so many rows the split kernel does it all in one launch (1,536 x 128 float: 9.6 us there, 7.1 here).
+constexpr int64_t kSplitRows = 1024;
 
 // Rows of one column workgroup: as many as keep its walk short; more rows than that become segments.
 constexpr int64_t kSegRows = 1024;
@@ -912,8 +998,10 @@ hipError_t launch_dropout(LayerType type, int64_t rows, int64_t cols, int64_t x_
         sh.chunks = (uint32_t)(n * sh.per_row);
         with_type(type, [&](auto t) {
             using T = decltype(t);
-            hipLaunchKernelGGL(dropout_kernel<T>, dim3((sh.chunks + 255) / 256), dim3(256), 0, s, static_cast<const T*>(x),
-                               static_cast<T*>(y), sh, drop);
+            with_flag(drop.threshold != 0, [&](auto on) {
+                hipLaunchKernelGGL((dropout_kernel<T, decltype(on)::value>), dim3((sh.chunks + 255) / 256), dim3(256), 0, s,
+                                   static_cast<const T*>(x), static_cast<T*>(y), sh, drop);
+            });
         });
     }
     return hipGetLastError();
@@ -928,11 +1016,13 @@ hipError_t launch_norm_forward(LayerType type, const NormArgs& args, hipStream_t
         with_flag(a.drop.threshold != 0, [&](auto drop) {
             constexpr bool D = decltype(drop)::value;
             const bool held = with_row_shape<T, true>(a.cols, [&](auto tpr, auto nv) {
-                constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, kRows = norm_threads(TPR) / TPR;
-                const int64_t blocks = std::min((a.rows + kRows - 1) / kRows, kForwardThreads / norm_threads(TPR));
-                hipLaunchKernelGGL((norm_forward_kernel<T, TPR, NV, D>), dim3((unsigned)blocks), dim3(norm_threads(TPR)), 0, s, a);
+                constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+                hipLaunchKernelGGL((norm_forward_kernel<T, TPR, NV, D>), dim3((unsigned)forward_blocks<TPR>(a.rows)), dim3(norm_threads(TPR)), 0, s, a);
             });
-            if (!held)
+            if (held) return;
+            if (a.cols < kChunk)
+                hipLaunchKernelGGL((norm_forward_walk_kernel<T, 1, D, false>), dim3((unsigned)std::min((a.rows + 255) / 256, kMaxBlocks)), dim3(256), 0, s, a);
+            else
                 hipLaunchKernelGGL((norm_forward_walk_kernel<T, 256, D, false>), dim3((unsigned)std::min(a.rows, kMaxBlocks)), dim3(256), 0, s, a);
         });
     });
