@@ -471,6 +471,23 @@ class Agents:
         W = [f64(w) for w in W]
         check(lib().epi_agents_set_weights(self._h, C.c_int32(agent), C.c_int32(int(target)), *[ptr(w, C.c_double) for w in W]))
 
+    def regularise(self, dropout: float = 0.0, eps: float = 1e-5, seed: int = 0) -> None:
+        """Layer norms, and dropout while learning, in both hidden layers of every network of the handle
+        (epi_agents_regularise): h = relu(norm(dropout(W x + b)))."""
+        check(lib().epi_agents_regularise(self._h, float(dropout), float(eps), int(seed)))
+
+    def norms(self, agent: int, target: bool = False):
+        """[gain1, bias1, gain2, bias2], [h] each, of one agent's layer norms."""
+        out = [np.zeros(self.hps[agent].hidden) for _ in range(4)]
+        check(lib().epi_agents_get_norm(self._h, C.c_int32(agent), C.c_int32(int(target)), *[ptr(w, C.c_double) for w in out]))
+        return out
+
+    def set_norms(self, agent: int, norms, target: bool = False) -> None:
+        norms = [f64(w) for w in norms]
+        if any(w.shape != (self.hps[agent].hidden,) for w in norms) or len(norms) != 4:
+            raise EpiError(_capi.EPI_ERR_BAD_ARGUMENT, "four arrays of %d values are needed" % self.hps[agent].hidden)
+        check(lib().epi_agents_set_norm(self._h, C.c_int32(agent), C.c_int32(int(target)), *[ptr(w, C.c_double) for w in norms]))
+
     def set_timing(self, on: bool):
         check(lib().epi_agents_set_timing(self._h, C.c_int32(int(on))))
 
@@ -873,6 +890,13 @@ class WorldToy:
                 nd.agent = DDQNAgent(nd.hyper_params, pool=self._pool, index=nd.idx)
             if self.device_transitions:
                 check(lib().epi_world_keep_transitions(self._h, C.c_int32(1)))
+
+    def regularise(self, dropout: float = 0.0, eps: float = 1e-5, seed: int = 0) -> None:
+        """Layer norms, and dropout while learning, in the networks of the nodes' agents (Agents.regularise)."""
+        if not self.learning:
+            raise EpiError(_capi.EPI_ERR_BAD_ARGUMENT, "the world has no learning agents (batch = 1 and learning = True)")
+        self._ensure_agents()
+        self._pool.regularise(dropout, eps, seed)
 
     # WorldToy.scala:157-162
     LEARNING_INTENSITY = {"India": 2, "Japan": 1, "Germany": 1}

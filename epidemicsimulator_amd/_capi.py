@@ -98,7 +98,7 @@ EXPORTED_SYMBOLS = [
     "epi_world_set_timing", "epi_world_kernel_time", "epi_world_result_buffers", "epi_world_step_packed", "epi_world_packed_buffer", "epi_world_destroy",
     "epi_agents_create", "epi_agents_destroy", "epi_agents_observe", "epi_agents_observe_world", "epi_agents_replay_size", "epi_agents_sample",
     "epi_agents_learn", "epi_agents_q_values", "epi_agents_get_weights", "epi_agents_set_weights",
-    "epi_agents_set_timing", "epi_agents_kernel_time",
+    "epi_agents_set_timing", "epi_agents_kernel_time", "epi_agents_regularise", "epi_agents_get_norm", "epi_agents_set_norm",
     "epi_dropout", "epi_layer_norm_forward", "epi_layer_norm_backward_workspace", "epi_layer_norm_backward",
 ]
 
@@ -169,6 +169,9 @@ def lib():
         L.epi_agents_set_weights.argtypes = [C.c_void_p, C.c_int32, C.c_int32] + [_PD] * 6
         L.epi_agents_set_timing.argtypes = [C.c_void_p, C.c_int32]
         L.epi_agents_kernel_time.argtypes = [C.c_void_p, C.POINTER(C.c_double), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]
+        L.epi_agents_regularise.argtypes = [C.c_void_p, C.c_double, C.c_double, C.c_int64]
+        L.epi_agents_get_norm.argtypes = [C.c_void_p, C.c_int32, C.c_int32] + [_PD] * 4
+        L.epi_agents_set_norm.argtypes = [C.c_void_p, C.c_int32, C.c_int32] + [_PD] * 4
         layer = C.POINTER(LayerDesc)
         L.epi_dropout.argtypes = [layer] + [C.c_void_p] * 3
         L.epi_layer_norm_forward.argtypes = [layer] + [C.c_void_p] * 7

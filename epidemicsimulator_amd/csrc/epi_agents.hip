@@ -24,6 +24,7 @@
 #include "../../include/epi.h"
 #include "epi_host.hpp"
 #include "epi_kernels.hpp"
+#include "epi_layers.hpp"
 #include "java_compat.hpp"
 
 #define EPI_API extern "C" __attribute__((visibility("default")))
@@ -240,6 +241,25 @@ __global__ void __launch_bounds__(1024) agents_forward_kernel(AgentsArgs a, cons
     }
 }
 
+// Prediction minus ddqnTarget (DDQNAgent.scala:37-47) of sample k of a slot, and the action it took.
+__device__ inline double td_error(const AgentsArgs& a, const AgentHyperDev& hp, int slot, int agent, int k, int& act) {
+    const double* q = a.Q + (((size_t)slot * 3 + 0) * a.Bp + k) * kOut;
+    const RingRec& rec = a.ring[a.ring_off[agent] + a.idx[(size_t)slot * a.Bp + k]];
+    act = rec.a;
+    double tgt;
+    if (rec.done) {
+        tgt = fmax(-hp.clip_q, fmin(hp.clip_q, rec.r));
+    } else {
+        const double* qn = a.Q + (((size_t)slot * 3 + 1) * a.Bp + k) * kOut;
+        const double* qt = a.Q + (((size_t)slot * 3 + 2) * a.Bp + k) * kOut;
+        int best = 0;  // zipWithIndex.maxBy(_._1): the first maximum
+        for (int o = 1; o < kOut; ++o)
+            if (qn[o] > qn[best]) best = o;
+        tgt = fmax(-hp.clip_q, fmin(hp.clip_q, rec.r + hp.gamma * qt[best]));
+    }
+    return q[act] - tgt;
+}
+
 // ddqnTarget (DDQNAgent.scala:37-47) and the backward pass of MLP.trainBatch (MLP.scala:44-58) for 64
 // samples.  The target equals the prediction in every component but the action taken, so err is zero there
 // and dh2(j) = W3(a)(j) * err(a).  dz = dh * relu(z) -- the activation's value, as the reference has it.
@@ -265,22 +285,8 @@ __global__ void __launch_bounds__(1024) agents_backward_kernel(AgentsArgs a, con
         int act = 0;
         if (lane < rows) {
             const size_t row = row0 + lane;
-            const double* q = a.Q + (((size_t)slot * 3 + 0) * a.Bp + k) * kOut;
-            const RingRec& rec = a.ring[a.ring_off[agent] + a.idx[row]];
-            act = rec.a;
+            err = td_error(a, hp, slot, agent, k, act);
             a.ACTd[row] = act;
-            double tgt;
-            if (rec.done) {
-                tgt = fmax(-hp.clip_q, fmin(hp.clip_q, rec.r));
-            } else {
-                const double* qn = a.Q + (((size_t)slot * 3 + 1) * a.Bp + k) * kOut;
-                const double* qt = a.Q + (((size_t)slot * 3 + 2) * a.Bp + k) * kOut;
-                int best = 0;  // zipWithIndex.maxBy(_._1): the first maximum
-                for (int o = 1; o < kOut; ++o)
-                    if (qn[o] > qn[best]) best = o;
-                tgt = fmax(-hp.clip_q, fmin(hp.clip_q, rec.r + hp.gamma * qt[best]));
-            }
-            err = q[act] - tgt;
             a.ERR[row] = err;
         }
         sh_err[lane] = err;
@@ -422,6 +428,155 @@ __global__ void __launch_bounds__(256) agents_grad_small_kernel(AgentsArgs a) {
     net[dst] -= hp.lr * clip_sym(acc * scale, hp.grad_clip);
 }
 
+// ---- networks with layer norms (epi_agents_regularise) ---------------------------------------------------
+// h = relu(norm(dropout(W x + b))) in both hidden layers: the linear layers below, and between them the kernels of
+// the layer operators, one set of rows and weights per (class, slot).  Pre-activations and normalised values are
+// [class][slot][Bp][Hp], class 0 first, so that dropout, which only the trained pass has, is one launch of its own.
+// The sums keep the order and the tiling of agents_forward_kernel; the derivative of the ReLU is 1 or 0.
+struct LinearStep {
+    int K;                  // inputs
+    size_t weights;         // offset in the network's image: [K][Hp]
+    long long bias;         // offset of [Hp], or -1
+    const double* in;       // [class][slot][Bp][Hp], or NULL: the sampled features
+    bool relu_in;
+    double* relu_out;       // [slot][Bp][Hp]: the inputs after the ReLU, class 0 (NULL: not kept)
+    const double* gate;     // [slot][Bp][Hp]: outputs where this is not above zero become zero (NULL: none)
+    double* out;            // [class][slot][Bp][Hp]
+};
+
+template <int kTile>
+__global__ void __launch_bounds__(1024) agents_linear_kernel(AgentsArgs a, const double* __restrict__ nets, LinearStep st) {
+    __shared__ double sh[kChunk * kLS];   // [unit][row]
+    const int slot = blockIdx.y, B = a.slot_rows[slot], groups = a.Bp / kTileRows;
+    const int cls = blockIdx.x / groups, k0 = (blockIdx.x % groups) * kTileRows;
+    if (k0 >= B) return;
+    const int H = a.nl.H, Hp = a.nl.Hp;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i0 = wave * kTile;
+    const int agent = a.slot_agent[slot];
+    const double* __restrict__ net = nets + ((size_t)agent * 2 + a.net_of_class[cls]) * a.nl.size();
+    const int rows = min(kTileRows, B - k0);
+    const size_t own = (size_t)slot * a.Bp + k0, row0 = (size_t)cls * gridDim.y * a.Bp + own;
+    double acc[kTile];
+    for (int c0 = 0; c0 < st.K; c0 += kChunk) {
+        const int cn = min(kChunk, st.K - c0);
+        __syncthreads();   // the previous chunk read by every wave
+        for (int idx = threadIdx.x; idx < kTileRows * kChunk; idx += blockDim.x) {
+            const int row = idx / kChunk, u = idx - row * kChunk;
+            double v = 0.0;
+            if (row < rows && u < cn) {
+                if (st.in) {
+                    v = st.in[(row0 + row) * Hp + c0 + u];
+                } else {
+                    const RingRec& rec = a.ring[a.ring_off[agent] + a.idx[own + row]];
+                    v = a.x_of_class[cls] ? rec.fs2[u] : rec.fs[u];
+                    if (cls == 0) a.X0d[(own + row) * kXStride + u] = v;
+                }
+                if (st.relu_in) v = v > 0 ? v : 0.0;
+                if (st.relu_out && cls == 0) st.relu_out[(own + row) * Hp + c0 + u] = v;
+            }
+            sh[u * kLS + row] = v;
+        }
+        __syncthreads();
+        if (i0 < H) ordered_tile(net + st.weights + (size_t)c0 * Hp + i0, Hp, sh + lane, cn, c0 == 0, acc);
+    }
+    if (i0 < H && st.bias >= 0) {
+#pragma unroll
+        for (int u = 0; u < kTile; ++u) acc[u] = acc[u] + net[st.bias + i0 + u];
+    }
+    for (int c0 = 0; c0 < H; c0 += kChunk) {
+        const int cn = min(kChunk, H - c0);
+        __syncthreads();
+        if (i0 >= c0 && i0 < c0 + kChunk && i0 < H) {
+#pragma unroll
+            for (int u = 0; u < kTile; ++u) sh[(i0 - c0 + u) * kLS + lane] = acc[u];
+        }
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < kTileRows * kChunk; idx += blockDim.x) {
+            const int row = idx / kChunk, u = idx - row * kChunk;
+            if (row < rows && u < cn) {
+                double v = sh[u * kLS + row];
+                if (st.gate && !(st.gate[(own + row) * Hp + c0 + u] > 0)) v = 0.0;
+                st.out[(row0 + row) * Hp + c0 + u] = v;
+            }
+        }
+    }
+}
+
+// Output layer of every class: relu(Y) W3 + b3, clamped; eight waves, one output each.  The activations of class 0 are
+// kept in H2 for the gradients.
+__global__ void __launch_bounds__(512) agents_output_kernel(AgentsArgs a, const double* __restrict__ nets, const double* Y) {
+    __shared__ double sh[kChunk * kLS];
+    const int slot = blockIdx.y, B = a.slot_rows[slot], groups = a.Bp / kTileRows;
+    const int cls = blockIdx.x / groups, k0 = (blockIdx.x % groups) * kTileRows;
+    if (k0 >= B) return;
+    const int H = a.nl.H, Hp = a.nl.Hp;
+    const int lane = threadIdx.x & 63, o = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int agent = a.slot_agent[slot];
+    const double* __restrict__ net = nets + ((size_t)agent * 2 + a.net_of_class[cls]) * a.nl.size();
+    const int rows = min(kTileRows, B - k0);
+    const size_t own = (size_t)slot * a.Bp + k0, row0 = (size_t)cls * gridDim.y * a.Bp + own;
+    double y = 0.0;
+    for (int c0 = 0; c0 < H; c0 += kChunk) {
+        const int cn = min(kChunk, H - c0);
+        __syncthreads();
+        for (int idx = threadIdx.x; idx < kTileRows * kChunk; idx += blockDim.x) {
+            const int row = idx / kChunk, u = idx - row * kChunk;
+            double v = 0.0;
+            if (row < rows && u < cn) {
+                v = Y[(row0 + row) * Hp + c0 + u];
+                v = v > 0 ? v : 0.0;
+                if (cls == 0) a.H2[(own + row) * Hp + c0 + u] = v;
+            }
+            sh[u * kLS + row] = v;
+        }
+        __syncthreads();
+        const double* __restrict__ W3 = net + a.nl.w3() + (size_t)o * Hp + c0;
+        int j = 0;
+        if (c0 == 0) { y = W3[0] * sh[lane]; j = 1; }
+#pragma unroll 16
+        for (; j < cn; ++j) y = y + W3[j] * sh[j * kLS + lane];
+    }
+    if (lane < rows) a.Q[(((size_t)slot * 3 + cls) * a.Bp + k0 + lane) * kOut + o] = clip_sym(y + net[a.nl.b3() + o], a.hyper[agent].clip_q);
+}
+
+// The gradient that reaches the second norm: (prediction - target) W3(action), where the unit was above zero.
+__global__ void __launch_bounds__(256) agents_output_gradient_kernel(AgentsArgs a, const double* __restrict__ nets, const double* Y, double* DY) {
+    __shared__ double sh_err[kTileRows];
+    __shared__ int sh_act[kTileRows];
+    const int slot = blockIdx.y, B = a.slot_rows[slot], k0 = blockIdx.x * kTileRows;
+    if (k0 >= B) return;
+    const int H = a.nl.H, Hp = a.nl.Hp, agent = a.slot_agent[slot];
+    const double* __restrict__ net = nets + (size_t)agent * 2 * a.nl.size();
+    const int rows = min(kTileRows, B - k0);
+    const size_t own = (size_t)slot * a.Bp + k0;
+    if ((int)threadIdx.x < rows) {
+        int act;
+        const double err = td_error(a, a.hyper[agent], slot, agent, k0 + threadIdx.x, act);
+        a.ACTd[own + threadIdx.x] = act;
+        a.ERR[own + threadIdx.x] = err;
+        sh_err[threadIdx.x] = err;
+        sh_act[threadIdx.x] = act;
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < rows * H; idx += blockDim.x) {
+        const int row = idx / H, u = idx - row * H;
+        const size_t at = (own + row) * Hp + u;
+        DY[at] = Y[at] > 0 ? net[a.nl.w3() + (size_t)sh_act[row] * Hp + u] * sh_err[row] : 0.0;
+    }
+}
+
+// Mean, clip and SGD of the gains and biases: [4][slots][H] sums in, [agent][2][4][Hp] parameters of the online
+// network out.
+__global__ void __launch_bounds__(256) agents_norm_step_kernel(AgentsArgs a, const double* sums, double* norm) {
+    const int slot = blockIdx.y, B = a.slot_rows[slot], H = a.nl.H, Hp = a.nl.Hp;
+    const int e = blockIdx.x * blockDim.x + threadIdx.x;
+    if (e >= 4 * H) return;
+    const int which = e / H, u = e - which * H, agent = a.slot_agent[slot];
+    const AgentHyperDev hp = a.hyper[agent];
+    const double g = sums[((size_t)which * gridDim.y + slot) * H + u] * (1.0 / (double)(B > 1 ? B : 1));
+    norm[((size_t)agent * 8 + which) * Hp + u] -= hp.lr * clip_sym(g, hp.grad_clip);
+}
+
 // DDQNAgent.observe -> ReplayBuffer.push (ReplayBuffer.scala:15-17): staged records into their ring slots.
 __global__ void __launch_bounds__(64) agents_push_kernel(RingRec* ring, const RingRec* staged, const long long* dst, int count) {
     const int k = blockIdx.x * blockDim.x + threadIdx.x;
@@ -506,6 +661,14 @@ struct epi_agents {
     std::vector<Replay> replay;
     std::vector<double> ema;
     DevBuf nets, hyper, H1, H2, Q, DZ2, DZ1, ERR, X0d, ACTd, ring, ring_off;
+    // networks with layer norms: parameters [n][2][4][Hp] (gains and biases of both layers), values [3][n][Bp][Hp], the
+    // gradient [n][Bp][Hp], sums [4][n][H], mean and deviation [2][2][n][Bp]; what each (class, slot) and layer works with
+    bool normed = false;
+    double norm_eps = 0.0, norm_dropout = 0.0;
+    int64_t norm_seed = 0;
+    std::vector<uint32_t> learns;   // learn steps taken by each agent: the dropout's counter
+    DevBuf norm, Z1, Z2, Y1, Y2, DY, norm_sums, norm_stats;
+    PinBuf set_index, set_used, set_ctr;
     PinBuf slot_agent, slot_rows, X, idx, loss, push_rec, push_dst, file_dst, q_in, q_out, q_act;
     std::vector<long long> h_ring_off;
     hipStream_t stream = nullptr;
@@ -614,6 +777,8 @@ int32_t agents_net_view(epi_agents* g, AgentsNetView* v) {
     v->nets = g->nets.as<double>(); v->net_stride = 2 * g->nl.size();
     v->clip_ptr = reinterpret_cast<const double*>(g->hyper.as<AgentHyperDev>()) + 2;   // AgentHyperDev::clip_q
     v->clip_stride = (int)(sizeof(AgentHyperDev) / sizeof(double));
+    v->norm = g->normed ? g->norm.as<double>() : nullptr;
+    v->norm_stride = (size_t)8 * g->nl.Hp; v->norm_eps = g->norm_eps;
     return EPI_OK;
 }
 }  // namespace epi
@@ -710,6 +875,95 @@ EPI_API int32_t epi_agents_sample(epi_agents* g, int32_t agent, int32_t n, int32
     return EPI_OK;
 }
 
+namespace {
+
+// The passes of learn for networks with layer norms: forward of the three classes, then the gradients of both layers'
+// pre-activations, gains and biases.  agents_grad_* take it from there.
+hipError_t norm_passes(epi_agents* g, const AgentsArgs& a, int slots) {
+    const int Bp = g->Bp, Hp = g->nl.Hp, H = g->nl.H;
+    const int32_t* agent = g->slot_agent.as<int32_t>();
+    const int32_t* rows = g->slot_rows.as<int32_t>();
+    int32_t* index = g->set_index.as<int32_t>();
+    int32_t* used = g->set_used.as<int32_t>();
+    uint32_t* ctr = g->set_ctr.as<uint32_t>();   // [layer][slot][2]
+    for (int cls = 0; cls < 3; ++cls)
+        for (int sl = 0; sl < slots; ++sl) {
+            index[cls * slots + sl] = agent[sl] * 2 + a.net_of_class[cls];
+            used[cls * slots + sl] = rows[sl];
+        }
+    for (int sl = 0; sl < slots; ++sl) {
+        const uint32_t call = g->learns[agent[sl]]++;
+        for (int layer = 0; layer < 2; ++layer) {
+            ctr[((size_t)layer * slots + sl) * 2] = 2 * call + layer;
+            ctr[((size_t)layer * slots + sl) * 2 + 1] = (uint32_t)agent[sl];
+        }
+    }
+    const size_t plane = (size_t)slots * Bp * Hp;   // one class
+    double *Z[2] = {g->Z1.as<double>(), g->Z2.as<double>()}, *Y[2] = {g->Y1.as<double>(), g->Y2.as<double>()};
+    double* DZ[2] = {g->DZ1.as<double>(), g->DZ2.as<double>()};
+    double* stats = g->norm_stats.as<double>();     // [layer][mean, rstd][slots * Bp] of class 0
+    auto norm_args = [&](int layer, int cls, int classes) {
+        NormArgs n{};
+        n.rows = (int64_t)classes * slots * Bp; n.cols = H;
+        n.x_stride = n.y_stride = n.dy_stride = Hp;
+        n.x = Z[layer] + cls * plane;
+        n.weight = g->norm.as<double>() + (size_t)(2 * layer) * Hp;
+        n.bias = g->norm.as<double>() + (size_t)(2 * layer + 1) * Hp;
+        n.eps = g->norm_eps;
+        n.drop = make_drop(cls == 0 ? g->norm_dropout : 0.0, g->norm_seed, 0, nullptr);
+        n.sets.count = classes * slots; n.sets.set_rows = Bp;
+        n.sets.set_index = g->set_index.on_device<int32_t>() + cls * slots;
+        n.sets.set_used = g->set_used.on_device<int32_t>() + cls * slots;
+        n.sets.weight_stride = (int64_t)4 * Hp;
+        if (cls == 0) {
+            n.sets.set_ctr = g->set_ctr.on_device<uint32_t>() + (size_t)layer * slots * 2;
+            n.mean = stats + (size_t)(2 * layer) * slots * Bp;
+            n.rstd = stats + (size_t)(2 * layer + 1) * slots * Bp;
+        }
+        return n;
+    };
+    const dim3 grid(3 * Bp / kTileRows, slots), own(Bp / kTileRows, slots), block(Hp / 16 * 64);
+    for (int layer = 0; layer < 2; ++layer) {
+        LinearStep st{};
+        st.K = layer ? H : kIn;
+        st.weights = layer ? g->nl.w2t() : g->nl.w1t();
+        st.bias = (long long)(layer ? g->nl.b2() : g->nl.b1());
+        st.in = layer ? Y[0] : nullptr;
+        st.relu_in = layer != 0;
+        st.relu_out = layer ? a.H1 : nullptr;
+        st.out = Z[layer];
+        hipLaunchKernelGGL(agents_linear_kernel<16>, grid, block, 0, g->stream, a, a.nets, st);
+        // the trained pass with its dropout, then the two passes of the target
+        for (int cls = 0; cls < 2; ++cls) {
+            NormArgs n = norm_args(layer, cls, cls + 1);
+            n.y = Y[layer] + cls * plane;
+            if (hipError_t e = launch_norm_forward(kF64, n, g->stream)) return e;
+        }
+    }
+    hipLaunchKernelGGL(agents_output_kernel, grid, dim3(512), 0, g->stream, a, a.nets, Y[1]);
+    hipLaunchKernelGGL(agents_output_gradient_kernel, own, dim3(256), 0, g->stream, a, a.nets, Y[1], g->DY.as<double>());
+    for (int layer = 1; layer >= 0; --layer) {
+        if (layer == 0) {
+            LinearStep st{};   // what reaches the first norm: W2 transposed times the second layer's, where h1 > 0
+            st.K = H;
+            st.weights = g->nl.w2();
+            st.bias = -1;
+            st.in = DZ[1];
+            st.gate = Y[0];
+            st.out = g->DY.as<double>();
+            hipLaunchKernelGGL(agents_linear_kernel<16>, own, block, 0, g->stream, a, a.nets, st);
+        }
+        NormArgs n = norm_args(layer, 0, 1);
+        n.dy = g->DY.p; n.dx = DZ[layer];
+        n.dweight = g->norm_sums.as<double>() + (size_t)(2 * layer) * slots * H;
+        n.dbias = g->norm_sums.as<double>() + (size_t)(2 * layer + 1) * slots * H;
+        if (hipError_t e = launch_norm_backward(kF64, n, g->stream)) return e;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace
+
 EPI_API int32_t epi_agents_learn(epi_agents* g, const int32_t* ids, int32_t count, const int32_t* batch,
                                  const int32_t* grad_accum, const int64_t* steps, double* loss, double* ema_loss) {
     if (!g || !batch || !grad_accum || !steps || !loss) return fail(EPI_ERR_BAD_ARGUMENT, "agents_learn: null argument");
@@ -757,11 +1011,17 @@ EPI_API int32_t epi_agents_learn(epi_agents* g, const int32_t* ids, int32_t coun
         const int Hp = g->nl.Hp, H = g->nl.H;
         if (g->timing) HIP_TRY(hipEventRecord(g->ev0, g->stream));
         const size_t lds = tile_lds_bytes();
-        // 16 hidden units per wave: tiles of 8 (twice the waves) measured slower on the default width
-        hipLaunchKernelGGL(agents_forward_kernel<16>, dim3(3 * Bp / kTileRows, slots), dim3(Hp / 16 * 64), lds, g->stream, a, a.nets);
-        hipLaunchKernelGGL(agents_backward_kernel<16>, dim3(Bp / kTileRows, slots), dim3(Hp / 16 * 64), lds, g->stream, a, a.nets);
+        if (g->normed) {
+            HIP_TRY(norm_passes(g, a, slots));
+        } else {
+            // 16 hidden units per wave: tiles of 8 (twice the waves) measured slower on the default width
+            hipLaunchKernelGGL(agents_forward_kernel<16>, dim3(3 * Bp / kTileRows, slots), dim3(Hp / 16 * 64), lds, g->stream, a, a.nets);
+            hipLaunchKernelGGL(agents_backward_kernel<16>, dim3(Bp / kTileRows, slots), dim3(Hp / 16 * 64), lds, g->stream, a, a.nets);
+        }
         hipLaunchKernelGGL(agents_grad_w2_kernel, dim3((H + kGradRows - 1) / kGradRows, slots), dim3(Hp), 0, g->stream, a);
         hipLaunchKernelGGL(agents_grad_small_kernel, dim3((17 * H + 9 + 255) / 256, slots), dim3(256), 0, g->stream, a);
+        if (g->normed)
+            hipLaunchKernelGGL(agents_norm_step_kernel, dim3((4 * H + 255) / 256, slots), dim3(256), 0, g->stream, a, g->norm_sums.as<double>(), g->norm.as<double>());
         HIP_TRY(hipGetLastError());
         // DDQNAgent.scala:59-61: the target network follows the updated online network
         for (int sl = 0; sl < slots; ++sl) {
@@ -771,6 +1031,10 @@ EPI_API int32_t epi_agents_learn(epi_agents* g, const int32_t* ids, int32_t coun
             if (steps[kk] % g->hp[id].target_update_every == 0) {
                 double* on = g->nets.as<double>() + ((size_t)id * 2) * g->nl.size();
                 HIP_TRY(hipMemcpyAsync(on + g->nl.size(), on, g->nl.size() * 8, hipMemcpyDeviceToDevice, g->stream));
+                if (g->normed) {
+                    double* pn = g->norm.as<double>() + (size_t)id * 8 * g->nl.Hp;
+                    HIP_TRY(hipMemcpyAsync(pn + 4 * g->nl.Hp, pn, (size_t)4 * g->nl.Hp * 8, hipMemcpyDeviceToDevice, g->stream));
+                }
             }
         }
         if (g->timing) HIP_TRY(hipEventRecord(g->ev1, g->stream));
@@ -817,6 +1081,10 @@ EPI_API int32_t epi_agents_q_values(epi_agents* g, const int32_t* ids, int32_t c
     ma.per_country = 1;
     ma.clip_ptr = reinterpret_cast<const double*>(g->hyper.as<AgentHyperDev>()) + 2;   // AgentHyperDev::clip_q
     ma.clip_stride = (int)(sizeof(AgentHyperDev) / sizeof(double));
+    if (g->normed) {
+        ma.norm = g->norm.as<double>(); ma.norm_stride = (size_t)8 * g->nl.Hp; ma.norm_eps = g->norm_eps;
+        ma.norm_offset = use_target ? (size_t)4 * g->nl.Hp : 0;
+    }
     ma.q_out = g->q_out.on_device<double>();
     ma.act_out = g->q_act.on_device<int32_t>();
     HIP_TRY(launch_mlp(ma, g->stream));
@@ -858,6 +1126,53 @@ EPI_API int32_t epi_agents_set_weights(epi_agents* g, int32_t agent, int32_t tar
     HIP_TRY(hipStreamSynchronize(g->stream));
     HIP_TRY(hipMemcpy(g->nets.as<double>() + ((size_t)agent * 2 + (target ? 1 : 0)) * g->nl.size(), img.data(),
                       g->nl.size() * 8, hipMemcpyHostToDevice));
+    return EPI_OK;
+}
+
+EPI_API int32_t epi_agents_regularise(epi_agents* g, double dropout, double eps, int64_t seed) {
+    if (!g) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: null handle");
+    if (!(dropout >= 0.0 && dropout < 1.0)) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: dropout %g outside [0,1)", dropout);
+    if (!(eps > 0.0) || !std::isfinite(eps)) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: eps %g is not a positive number", eps);
+    if (int32_t rc = use_device(g->device)) return rc;
+    HIP_TRY(hipStreamSynchronize(g->stream));
+    const size_t n = (size_t)g->n, H = (size_t)g->nl.H, Hp = (size_t)g->nl.Hp, plane = n * g->Bp * Hp * 8;
+    std::vector<double> params(n * 8 * Hp, 0.0);   // gains one, biases zero, nothing behind the last unit
+    for (size_t k = 0; k < n * 4; ++k)
+        for (size_t u = 0; u < H; ++u) params[k * 2 * Hp + u] = 1.0;
+    g->normed = false;   // until everything is there
+    HIP_TRY(g->Z1.ensure(3 * plane)); HIP_TRY(g->Z2.ensure(3 * plane));
+    HIP_TRY(g->Y1.ensure(3 * plane)); HIP_TRY(g->Y2.ensure(3 * plane));
+    HIP_TRY(g->DY.ensure(plane)); HIP_TRY(g->norm_sums.ensure(4 * n * H * 8));
+    HIP_TRY(g->norm_stats.ensure(4 * n * g->Bp * 8));
+    HIP_TRY(g->set_index.ensure(3 * n * 4)); HIP_TRY(g->set_used.ensure(3 * n * 4)); HIP_TRY(g->set_ctr.ensure(4 * n * 4));
+    HIP_TRY(g->norm.upload(params));
+    g->learns.assign(n, 0);
+    g->norm_dropout = dropout; g->norm_eps = eps; g->norm_seed = seed;
+    g->normed = true;
+    return EPI_OK;
+}
+
+EPI_API int32_t epi_agents_get_norm(epi_agents* g, int32_t agent, int32_t target, double* gain1, double* bias1, double* gain2, double* bias2) {
+    if (!g || agent < 0 || agent >= g->n) return fail(EPI_ERR_BAD_ARGUMENT, "agents_get_norm: bad argument");
+    if (!g->normed) return fail(EPI_ERR_BAD_ARGUMENT, "agents_get_norm: the networks have no layer norms (epi_agents_regularise)");
+    if (int32_t rc = use_device(g->device)) return rc;
+    HIP_TRY(hipStreamSynchronize(g->stream));
+    double* out[4] = {gain1, bias1, gain2, bias2};
+    for (int k = 0; k < 4; ++k)
+        if (out[k])
+            HIP_TRY(hipMemcpy(out[k], g->norm.as<double>() + ((size_t)agent * 8 + (target ? 4 : 0) + k) * g->nl.Hp, (size_t)g->nl.H * 8, hipMemcpyDeviceToHost));
+    return EPI_OK;
+}
+
+EPI_API int32_t epi_agents_set_norm(epi_agents* g, int32_t agent, int32_t target, const double* gain1, const double* bias1, const double* gain2,
+                                    const double* bias2) {
+    if (!g || agent < 0 || agent >= g->n || !gain1 || !bias1 || !gain2 || !bias2) return fail(EPI_ERR_BAD_ARGUMENT, "agents_set_norm: bad argument");
+    if (!g->normed) return fail(EPI_ERR_BAD_ARGUMENT, "agents_set_norm: the networks have no layer norms (epi_agents_regularise)");
+    if (int32_t rc = use_device(g->device)) return rc;
+    HIP_TRY(hipStreamSynchronize(g->stream));
+    const double* in[4] = {gain1, bias1, gain2, bias2};
+    for (int k = 0; k < 4; ++k)
+        HIP_TRY(hipMemcpy(g->norm.as<double>() + ((size_t)agent * 8 + (target ? 4 : 0) + k) * g->nl.Hp, in[k], (size_t)g->nl.H * 8, hipMemcpyHostToDevice));
     return EPI_OK;
 }
 

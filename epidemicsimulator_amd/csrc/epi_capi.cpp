@@ -1962,6 +1962,7 @@ EPI_API int32_t epi_world_rollout_greedy(epi_world* w, epi_agents* agents, int32
     if (agents) {
         ma.nl = view.nl; ma.nets = view.nets; ma.net_stride = view.net_stride; ma.per_country = 1;
         ma.clip_ptr = view.clip_ptr; ma.clip_stride = view.clip_stride; ma.clip_q = 0.0;
+        ma.norm = view.norm; ma.norm_stride = view.norm_stride; ma.norm_eps = view.norm_eps;
     } else {
         w->mlp.fill(ma);
     }

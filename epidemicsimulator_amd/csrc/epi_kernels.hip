@@ -2102,6 +2102,90 @@ __global__ __launch_bounds__(MLP_TILE_THREADS) void mlp_tile_kernel(const MlpArg
     }
 }
 
+// Sum over a workgroup of at most four waves; every thread gets it.  `sh` holds four doubles and is free again
+// after the call's second barrier.
+__device__ inline double group_sum(double v, double* sh) {
+    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = sh[0];
+    for (int w = 1; w < (int)(blockDim.x >> 6); ++w) s += sh[w];
+    __syncthreads();
+    return s;
+}
+
+// Greedy action of networks with layer norms (regularised learners): relu(norm(W x + b)) twice, then the outputs, the
+// clamp and the first maximum as in mlp_greedy_kernel.  A workgroup takes one state, a thread one hidden unit; at most
+// 256 of them, so the norm's sums are two barriers each and the second layer's weights come coalesced from L2.  A world
+// of six countries asks six workgroups, which run side by side: the time is that of one chain of loads.
+__global__ __launch_bounds__(256) void mlp_norm_kernel(const MlpArgs a) {
+    __shared__ double sh_x[8], sh_y[8], sh_sum[4], sh_h[2][256];
+    const int H = a.nl.H, Hp = a.nl.Hp, tid = threadIdx.x;
+    const int e = blockIdx.x, c = blockIdx.y;
+    const size_t nidx = (size_t)(a.net_index ? a.net_index[c] : c);
+    const double* __restrict__ net = a.nets + nidx * a.net_stride + a.net_offset;
+    const double* __restrict__ norm = a.norm + nidx * a.norm_stride + a.norm_offset;
+    if (tid == 0) {
+        double s, i, r, d, v, cap;
+        int32_t t, tmax;
+        if (a.st) {
+            const size_t idx = (size_t)e * a.npad + c;
+            s = (double)a.st[0 * a.plane + idx]; i = (double)a.st[1 * a.plane + idx];
+            r = (double)a.st[2 * a.plane + idx]; d = (double)a.st[3 * a.plane + idx];
+            v = (double)a.st[4 * a.plane + idx];
+            cap = a.cap[idx]; t = a.tcur[idx]; tmax = a.state_t_max;
+        } else {
+            const epi_state& st = a.states[(size_t)e * a.n + c];
+            s = st.s; i = st.i; r = st.r; d = st.d; v = st.v; cap = st.hosp_cap; t = st.t; tmax = st.t_max;
+        }
+        const double N = fmax(1.0, s + i + r + d);
+        sh_x[0] = s / N; sh_x[1] = i / N; sh_x[2] = r / N; sh_x[3] = d / N; sh_x[4] = v / N;
+        sh_x[5] = i / fmax(1.0, cap);
+        sh_x[6] = (double)t / (double)(tmax > 1 ? tmax : 1);
+    }
+    __syncthreads();
+    for (int layer = 0; layer < 2; ++layer) {
+        // the images are padded to Hp = blockDim.x units
+        double z;
+        if (layer == 0) {
+            z = net[a.nl.w1t() + tid] * sh_x[0];
+            for (int k = 1; k < 7; ++k) z = z + net[a.nl.w1t() + (size_t)k * Hp + tid] * sh_x[k];
+            z = z + net[a.nl.b1() + tid];
+        } else {
+            z = net[a.nl.w2t() + tid] * sh_h[0][0];
+#pragma unroll 16
+            for (int k = 1; k < H; ++k) z = z + net[a.nl.w2t() + (size_t)k * Hp + tid] * sh_h[0][k];
+            z = z + net[a.nl.b2() + tid];
+        }
+        const double m = group_sum(tid < H ? z : 0.0, sh_sum) / H;
+        const double u = tid < H ? z - m : 0.0;
+        const double var = group_sum(u * u, sh_sum) / H;
+        const double y = u * (1.0 / sqrt(var + a.norm_eps)) * norm[(2 * layer) * Hp + tid] + norm[(2 * layer + 1) * Hp + tid];
+        sh_h[layer][tid] = y > 0 ? y : 0.0;
+        __syncthreads();
+    }
+    if (tid < 8) {
+        const double* __restrict__ W3 = net + a.nl.w3() + (size_t)tid * Hp;
+        double y = W3[0] * sh_h[1][0];
+        for (int k = 1; k < H; ++k) y = y + W3[k] * sh_h[1][k];
+        y = y + net[a.nl.b3() + tid];
+        const double clip = a.clip_ptr ? a.clip_ptr[nidx * a.clip_stride] : a.clip_q;
+        if (isfinite(clip)) y = fmax(-clip, fmin(clip, y));
+        sh_y[tid] = y;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        const size_t row = (size_t)e * a.n + c;
+        int best = 0;
+        for (int o = 1; o < 8; ++o)
+            if (sh_y[o] > sh_y[best]) best = o;
+        if (a.act_episode) a.act_episode[(size_t)e * a.npad + c] = (int8_t)best;
+        if (a.act_out) a.act_out[row] = best;
+        if (a.q_out)
+            for (int o = 0; o < 8; ++o) a.q_out[row * 8 + o] = sh_y[o];
+    }
+}
+
 template <int ROWS>
 static hipError_t launch_mlp_rows(const MlpArgs& a, int live, hipStream_t s) {
     const int H = a.nl.H;
@@ -2119,6 +2203,11 @@ hipError_t launch_mlp(const MlpArgs& a, hipStream_t s) {
     if (a.rows <= 0) return hipSuccess;
     const int H = a.nl.H;
     if (H < 1 || H > MLP_MAXH || a.nl.Hp < H || a.nl.Hp % 64 != 0) return hipErrorInvalidValue;
+    if (a.norm) {
+        if (!a.per_country || a.nl.Hp > 256) return hipErrorInvalidValue;
+        hipLaunchKernelGGL(mlp_norm_kernel, dim3((unsigned)a.count, (unsigned)a.n), dim3((unsigned)a.nl.Hp), 0, s, a);
+        return hipGetLastError();
+    }
     const int live = a.per_country ? a.count : a.rows;   // states that share a network
     if (live >= 4 * MLP_TILE_ROWS && H == a.nl.Hp && (H == 64 || H == 128)) {   // a large batch on one network
         const dim3 grid((unsigned)((live + MLP_TILE_ROWS - 1) / MLP_TILE_ROWS), a.per_country ? (unsigned)a.n : 1u);

@@ -180,6 +180,11 @@ struct MlpArgs {
     double clip_q;            // clamp of the outputs (MLP.scala:21), used when clip_ptr == NULL
     const double* clip_ptr;   // per-country clamp: clip_ptr[c * clip_stride]
     int clip_stride;
+    // Layer norms of both hidden layers, before the ReLU (regularised learners; per_country): [4][Hp] = gains and
+    // biases of the first, then of the second, in network order like `nets`; NULL = plain networks.
+    const double* norm;
+    size_t norm_stride, norm_offset;
+    double norm_eps;
     int8_t* act_episode;  // [count][npad] (when st != NULL)
     int32_t* act_out;     // [rows] optional
     double* q_out;        // [rows][8] optional
@@ -276,6 +281,8 @@ struct AgentsNetView {
     NetLayout nl;
     const double* nets; size_t net_stride;
     const double* clip_ptr; int clip_stride;
+    const double* norm; size_t norm_stride;   // NULL: plain networks
+    double norm_eps;
 };
 }  // namespace epi
 struct epi_agents;

@@ -21,7 +21,7 @@ struct DropArgs {
 };
 DropArgs make_drop(double p, int64_t seed, int64_t offset, const int64_t* offset_dev);
 
-// Weights of several networks in one call (one set of rows each): rows k * set_rows .. + set_used[k] - 1 belong to
+// Weights of several networks in one call, of doubles (one set of rows each): rows k * set_rows .. + set_used[k] - 1 belong to
 // set k and use weight / bias number set_index[k]; the rows behind set_used[k] are neither read nor written.
 // set_ctr[2 k .. 2 k + 1] replaces the dropout offset of set k, and its rows count from zero.
 struct NormSets {

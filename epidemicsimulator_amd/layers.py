@@ -16,6 +16,19 @@ import torch
 from . import _capi
 from . import _layers
 
+
+def _hip_runtimes():
+    """The HIP runtimes this process has loaded.  torch brings one of its own: libepi.so uses it where torch came first,
+    and loads the system's where it came first itself; devices, streams and memory of two are strangers to each other."""
+    with open("/proc/self/maps") as maps:
+        return sorted({line.split(None, 5)[5].strip() for line in maps if "libamdhip64.so" in line})
+
+
+_capi.lib()
+if len(_hip_runtimes()) > 1:
+    raise ImportError("two HIP runtimes are loaded (%s): import torch, or epidemicsimulator_amd.layers, before the first "
+                      "call into libepi.so" % ", ".join(_hip_runtimes()))
+
 __all__ = ["dropout", "layer_norm", "layer_norm_forward", "layer_norm_backward"]
 
 _layers.bind({name: C.cast(getattr(_capi.lib(), name), C.c_void_p).value for name in (

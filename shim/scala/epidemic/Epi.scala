@@ -81,6 +81,9 @@ object Epi {
   val agentsQValues = fn("epi_agents_q_values", JAVA_INT, ADDRESS, ADDRESS, JAVA_INT, ADDRESS, JAVA_INT, ADDRESS, ADDRESS)
   val agentsGetWeights = fn("epi_agents_get_weights", JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
   val agentsSetWeights = fn("epi_agents_set_weights", JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
+  val agentsRegularise = fn("epi_agents_regularise", JAVA_INT, ADDRESS, JAVA_DOUBLE, JAVA_DOUBLE, JAVA_LONG)
+  val agentsGetNorm = fn("epi_agents_get_norm", JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
+  val agentsSetNorm = fn("epi_agents_set_norm", JAVA_INT, ADDRESS, JAVA_INT, JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
   val agentsSetTiming = fn("epi_agents_set_timing", JAVA_INT, ADDRESS, JAVA_INT)
   val agentsKernelTime = fn("epi_agents_kernel_time", JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS)
   val dropout = fn("epi_dropout", JAVA_INT, ADDRESS, ADDRESS, ADDRESS, ADDRESS)

@@ -6,8 +6,10 @@ import inspect
 import numpy as np
 import pytest
 
-from epidemicsimulator_amd import _capi
-from oracle import layers_ref as R
+torch = pytest.importorskip("torch")   # before libepi.so: the two share torch's HIP runtime
+
+from epidemicsimulator_amd import _capi  # noqa: E402
+from oracle import layers_ref as R  # noqa: E402
 
 BAD, DEVICE, UNSUPPORTED = _capi.EPI_ERR_BAD_ARGUMENT, _capi.EPI_ERR_DEVICE, _capi.EPI_ERR_UNSUPPORTED
 
@@ -161,7 +163,6 @@ def test_valid_arguments_reach_the_device_check():
 
 
 def test_python_refuses_tensors_that_are_not_on_a_gpu():
-    torch = pytest.importorskip("torch")
     from epidemicsimulator_amd import layers
     x = torch.zeros(3, 8)
     for f in (lambda: layers.dropout(x, 0.1, 1), lambda: layers.layer_norm(x), lambda: layers.layer_norm_forward(x),
@@ -169,6 +170,17 @@ def test_python_refuses_tensors_that_are_not_on_a_gpu():
         with pytest.raises(_capi.EpiError) as e:
             f()
         assert e.value.status == BAD
+
+
+def test_two_hip_runtimes_are_refused():
+    """libepi.so loaded before torch: the binding says so instead of mixing the two (in a process of its own)."""
+    import subprocess
+    import sys
+    code = ("import epidemicsimulator_amd as E; E.lib()\n"
+            "try:\n    from epidemicsimulator_amd import layers\n"
+            "except ImportError as e:\n    assert 'two HIP runtimes' in str(e)\n"
+            "else:\n    assert len(layers._hip_runtimes()) == 1\n")
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
 
 
 def test_public_names_are_documented():
