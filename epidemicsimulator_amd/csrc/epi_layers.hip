@@ -355,7 +355,9 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T
 
 // ---- layer norm, forward: rows that fit the registers of their threads ---------------------------------
 // TPR threads hold a row, NV chunks of eight columns each: it is read once, and while it is worked on the next row
-// is on its way.  TPR <= 64: 256 / TPR rows side by side in a workgroup, no barrier; else a row per workgroup.
+// is on its way.  TPR <= 64: 256 / TPR rows side by side in a workgroup, no barrier; else a row per workgroup.  Bound by
+// memory: 819,200 x 128 bfloat16 take 77 us (5.4 TB/s, a large copy reaches 5.0 to 5.4), 79 with dropout; 16,384 x
+// 4,096 bfloat16 47 us (5.7 TB/s, part of it from the caches); 24,576 x 128 float 6.6 us, of which 2.5 are the launch.
 constexpr int norm_threads(int tpr) { return tpr > 64 ? tpr : 256; }
 
 // The chunk of a row of at least eight columns that a thread works on.  Where the row's end cuts it, it is moved back
@@ -416,6 +418,9 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArg
     using A = wide_t<T>;
     constexpr int kRows = norm_threads(TPR) / TPR;
     constexpr bool kHold = NV == 1 && sizeof(T) < 8;   // registers for the weights
+    // registers for the next row, where they are left: 1,024 threads have 128 each (1,021 x 20,000 float with dropout:
+    // 43.7 us with the next row's and spills, 38.4 without; without dropout 36.7 with and 36.6 without)
+    constexpr bool kAhead = TPR < 1024 || (DROP ? NV < 4 && NV * sizeof(T) <= 8 : NV * sizeof(T) <= 16);
     __shared__ A lds[kRowLds<TPR, 2>];
     int flip = 0;
     const int t = threadIdx.x % TPR, cols = (int)a.cols;
@@ -446,7 +451,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArg
 #pragma unroll
         for (int v = 0; v < NV; ++v) widen_chunk(raw[v], h[v]);
         const int64_t next = row + step;
-        if (next < a.rows) fetch(next);
+        if (kAhead && next < a.rows) fetch(next);
         A s[1] = {0};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -491,6 +496,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArg
             put_part<T, kChunk>(y + p.col, o.w);
         }
         row = next;
+        if (!kAhead && row < a.rows) fetch(row);
     }
 }
 
@@ -707,7 +713,9 @@ __global__ __launch_bounds__(256) void norm_backward_split_kernel(NormArgs a, Sp
 // workgroup, in registers; at the end the workgroup's rows are summed (lanes, then waves, in a fixed order) and
 // one partial row of both gradients is left in the workspace for norm_reduce_kernel.  x and dy stay as they were
 // loaded: u and g are formed twice, before and after the row's two means, which is cheaper than the registers of a
-// widened copy.
+// widened copy.  Bound by memory while a wave's registers hold a row: 819,200 x 128 bfloat16 take 122 us with the
+// reduction (5.1 TB/s over x, dy and dx), 16,384 x 4,096 bfloat16 91 us (4.4 TB/s: 5 of them are the reduction of 512
+// partial rows); beyond 8,192 columns by the registers (6,000 x 16,000 bfloat16: 171 us, 3.4 TB/s).
 template <class T, int TPR, int NV, bool DROP>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormArgs a) {
     using A = wide_t<T>;

@@ -6,8 +6,10 @@
 // The entry points are handed over as addresses, so this module needs no libepi.so of its own beside the one that is
 // loaded already.
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
 #include <string>
@@ -17,7 +19,7 @@
 
 namespace py = pybind11;
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 namespace {
@@ -131,22 +133,24 @@ Tensor run_dropout(const Tensor& t, const Drop& drop) {
     return y;
 }
 
-std::tuple<Tensor, Tensor, Tensor> run_forward(const Tensor& t, const Tensor& w, const Tensor& b, double eps, const Drop& drop, bool stats) {
+// (y, stats): stats holds the rows' means, then their 1 / deviation
+std::pair<Tensor, Tensor> run_forward(const Tensor& t, const Tensor& w, const Tensor& b, double eps, const Drop& drop, bool want_stats) {
     const auto [x, stride] = rows_of(t);
     const Tensor weight = vector_of("weight", w, x), bias = vector_of("bias", b, x);
     epi_layer_desc d = desc_of(x, eps, drop);
-    Tensor y = empty_like_rows(x), mean, rstd;
+    Tensor y = empty_like_rows(x), stats;
     d.x_stride = stride; d.y_stride = d.cols;
-    if (stats) {
-        const auto wide = x.options().dtype(d.dtype == EPI_F64 ? at::kDouble : at::kFloat);
-        mean = at::empty({d.rows}, wide);
-        rstd = at::empty({d.rows}, wide);
+    void *mean = nullptr, *rstd = nullptr;
+    if (want_stats) {
+        stats = at::empty({2, d.rows}, x.options().dtype(d.dtype == EPI_F64 ? at::kDouble : at::kFloat));
+        mean = stats.data_ptr();
+        rstd = static_cast<char*>(mean) + d.rows * stats.element_size();
     }
-    check(lib.forward(&d, x.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), ptr(mean), ptr(rstd), stream_of(x)));
-    return {y, mean, rstd};
+    check(lib.forward(&d, x.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), mean, rstd, stream_of(x)));
+    return {y, stats};
 }
 
-std::tuple<Tensor, Tensor, Tensor> run_backward(const Tensor& g, const Tensor& t, const Tensor& w, const Tensor& mean, const Tensor& rstd,
+std::tuple<Tensor, Tensor, Tensor> run_backward(const Tensor& g, const Tensor& t, const Tensor& w, const void* mean, const void* rstd,
                                                 const Drop& drop, bool want_x, bool want_weight, bool want_bias) {
     const auto [x, stride] = rows_of(t);
     const auto [dy, dy_stride] = rows_of(g);
@@ -160,70 +164,100 @@ std::tuple<Tensor, Tensor, Tensor> run_backward(const Tensor& g, const Tensor& t
     size_t need = 0;
     if (want_weight || want_bias) check(lib.workspace(&d, &need));
     if (need) work = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
-    check(lib.backward(&d, x.data_ptr(), dy.data_ptr(), ptr(weight), ptr(mean), ptr(rstd), ptr(dx), ptr(dweight), ptr(dbias),
-                       ptr(work), need, stream_of(x)));
+    check(lib.backward(&d, x.data_ptr(), dy.data_ptr(), ptr(weight), mean, rstd, ptr(dx), ptr(dweight), ptr(dbias), ptr(work), need,
+                       stream_of(x)));
     return {dx, dweight, dbias};
 }
 
 // ---- autograd -----------------------------------------------------------------------------------------------
 // Gradients are values only: asked to differentiate them again (create_graph), the node behind them refuses.
-variable_list once(variable_list grads) {
-    if (!at::GradMode::is_enabled()) return grads;
+variable_list once(variable_list grads, bool again) {
+    if (!again) return grads;
     for (auto& g : grads)
         if (g.defined()) g = g.detach().requires_grad_(true);
     auto error = std::make_shared<torch::autograd::DelayedError>("the gradients of layer operators cannot be differentiated again", (int)grads.size());
     return (*error)(std::move(grads));
 }
-void keep_drop(AutogradContext* ctx, const Drop& drop) {
-    ctx->saved_data["p"] = drop.p;
-    ctx->saved_data["seed"] = drop.seed;
-    ctx->saved_data["offset"] = drop.offset;
-}
-Drop kept_drop(AutogradContext* ctx, const Tensor& offset_dev) {
-    Drop d;
-    d.p = ctx->saved_data["p"].toDouble();
-    d.seed = ctx->saved_data["seed"].toInt();
-    d.offset = ctx->saved_data["offset"].toInt();
-    d.offset_dev = offset_dev;
-    return d;
-}
 
-struct DropoutNode : torch::autograd::Function<DropoutNode> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Drop& drop) {
-        keep_drop(ctx, drop);
-        ctx->save_for_backward({drop.offset_dev});
-        return run_dropout(x, drop);
-    }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        variable_list out(2);
+// The nodes of the graph, with what their backward passes need.
+struct DropoutNode : torch::autograd::Node {
+    Drop drop;
+    SavedVariable offset_dev;
+    variable_list apply(variable_list&& grads) override {
+        const bool again = at::GradMode::is_enabled();
+        at::AutoGradMode off(false);
+        variable_list out(1);
         if (grads[0].defined()) {
-            at::AutoGradMode off(false);
-            out[0] = run_dropout(grads[0], kept_drop(ctx, saved[0]));
+            Drop d = drop;
+            d.offset_dev = offset_dev.unpack();
+            out[0] = run_dropout(grads[0], d);
         }
-        return once(std::move(out));
+        at::AutoGradMode on(again);
+        return once(std::move(out), again);
     }
+    void release_variables() override { offset_dev.reset_data(); }
+    std::string name() const override { return "EpiDropoutBackward"; }
 };
 
-struct NormNode : torch::autograd::Function<NormNode> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps, const Drop& drop) {
-        auto [y, mean, rstd] = run_forward(x, w, b, eps, drop, true);
-        keep_drop(ctx, drop);
-        ctx->save_for_backward({x, w, mean, rstd, drop.offset_dev});
-        return y;
-    }
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        variable_list out(5);
+struct NormNode : torch::autograd::Node {
+    Drop drop;
+    SavedVariable x, weight, stats, offset_dev;
+    variable_list apply(variable_list&& grads) override {
+        const bool again = at::GradMode::is_enabled();
+        at::AutoGradMode off(false);
+        variable_list out(3);
         if (grads[0].defined()) {
-            at::AutoGradMode off(false);
+            const Tensor s = stats.unpack();
+            Drop d = drop;
+            d.offset_dev = offset_dev.unpack();
+            const char* mean = static_cast<const char*>(s.data_ptr());
             std::tie(out[0], out[1], out[2]) =
-                run_backward(grads[0], saved[0], saved[1], saved[2], saved[3], kept_drop(ctx, saved[4]), ctx->needs_input_grad(0),
-                             ctx->needs_input_grad(1), ctx->needs_input_grad(2));
+                run_backward(grads[0], x.unpack(), weight.unpack(), mean, mean + s.size(1) * s.element_size(), d, task_should_compute_output(0),
+                             task_should_compute_output(1), task_should_compute_output(2));
         }
-        return once(std::move(out));
+        at::AutoGradMode on(again);
+        return once(std::move(out), again);
     }
+    void release_variables() override {
+        x.reset_data(); weight.reset_data(); stats.reset_data(); offset_dev.reset_data();
+    }
+    std::string name() const override { return "EpiLayerNormBackward"; }
 };
+
+template <class N>
+std::shared_ptr<N> new_node() { return std::shared_ptr<N>(new N(), torch::autograd::deleteNode); }
+
+Tensor record_dropout(const Tensor& x, const Drop& drop) {
+    Tensor y;
+    {
+        at::AutoGradMode off(false);
+        y = run_dropout(x, drop);
+    }
+    auto node = new_node<DropoutNode>();
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    node->drop = drop;
+    node->drop.offset_dev.reset();
+    node->offset_dev = SavedVariable(drop.offset_dev, false);
+    torch::autograd::set_history(y, node);
+    return y;
+}
+Tensor record_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps, const Drop& drop) {
+    std::pair<Tensor, Tensor> r;
+    {
+        at::AutoGradMode off(false);
+        r = run_forward(x, w, b, eps, drop, true);
+    }
+    auto node = new_node<NormNode>();
+    node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
+    node->drop = drop;
+    node->drop.offset_dev.reset();
+    node->x = SavedVariable(x, false);
+    node->weight = SavedVariable(w, false);
+    node->stats = SavedVariable(r.second, false);
+    node->offset_dev = SavedVariable(drop.offset_dev, false);
+    torch::autograd::set_history(r.first, node);
+    return r.first;
+}
 
 // ---- what Python calls ------------------------------------------------------------------------------------
 // Any integer, taken modulo 2^64.
@@ -253,15 +287,15 @@ Tensor dropout(const py::handle& x_, double p, const py::handle& seed, const py:
     const Drop drop = drop_of(p, seed, offset);
     py::gil_scoped_release free;
     check_x("x", x);
-    return at::GradMode::is_enabled() && wants(x) ? DropoutNode::apply(x, drop) : run_dropout(x, drop);
+    return at::GradMode::is_enabled() && wants(x) ? record_dropout(x, drop) : run_dropout(x, drop);
 }
 Tensor layer_norm(const py::handle& x_, const py::handle& w_, const py::handle& b_, double eps, double p, const py::handle& seed, const py::handle& offset) {
     const Tensor x = tensor_of("x", x_, false), w = tensor_of("weight", w_, true), b = tensor_of("bias", b_, true);
     const Drop drop = drop_of(p, seed, offset);
     py::gil_scoped_release free;
     check_x("x", x);
-    if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) return NormNode::apply(x, w, b, eps, drop);
-    return std::get<0>(run_forward(x, w, b, eps, drop, false));
+    if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) return record_norm(x, w, b, eps, drop);
+    return run_forward(x, w, b, eps, drop, false).first;
 }
 std::tuple<Tensor, Tensor, Tensor> layer_norm_forward(const py::handle& x_, const py::handle& w_, const py::handle& b_, double eps, double p,
                                                       const py::handle& seed, const py::handle& offset) {
@@ -270,7 +304,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_forward(const py::handle& x_, cons
     py::gil_scoped_release free;
     at::AutoGradMode off(false);
     check_x("x", x);
-    return run_forward(x, w, b, eps, drop, true);
+    const auto [y, stats] = run_forward(x, w, b, eps, drop, true);
+    return {y, stats.select(0, 0), stats.select(0, 1)};
 }
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const py::handle& dy_, const py::handle& x_, const py::handle& w_, const py::handle& mean_,
                                                        const py::handle& rstd_, double p, const py::handle& seed, const py::handle& offset) {
@@ -288,7 +323,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const py::handle& dy_, co
     for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"mean", mean}, {"rstd", rstd}})
         if (t.device() != x.device() || t.scalar_type() != wide || !t.is_contiguous() || t.numel() != rows)
             refuse(std::string(name) + " is not the forward pass's: " + str(rows) + " numbers of " + str(wide) + " on " + str(x.device()));
-    return run_backward(dy, x, w, mean, rstd, drop, true, true, true);
+    return run_backward(dy, x, w, mean.data_ptr(), rstd.data_ptr(), drop, true, true, true);
 }
 
 template <class F>
