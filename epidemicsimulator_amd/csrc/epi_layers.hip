@@ -961,8 +961,12 @@ int64_t backward_blocks(int64_t rows) {
 // Up to so many rows the split kernel does it all in one launch (1,536 x 128 float: 9.6 us there, 7.1 here).
 constexpr int64_t kSplitRows = 1024;
 
-// Rows side by side in a workgroup of the kernels for several networks at once, whose rows have up to 256 columns.
-constexpr int kSetRows = 8;
+// Threads of a row in the kernels for several networks at once, whose rows have up to 256 columns: one chunk each.
+template <class F>
+void with_set_shape(int64_t cols, F f) {
+    if (cols <= 128) f(int_c<16>{});
+    else f(int_c<32>{});
+}
 
 // Rows of one column workgroup: as many as keep its walk short; more rows than that become segments.
 constexpr int64_t kSegRows = 1024;
@@ -1023,10 +1027,11 @@ hipError_t launch_norm_forward(LayerType type, const NormArgs& args, hipStream_t
     NormArgs a = args;
     a.inv_cols = 1.0 / (double)a.cols;
     if (a.sets.count) {
-        const dim3 grid((unsigned)std::min((a.rows + kSetRows - 1) / kSetRows, kMaxBlocks));
-        with_flag(a.drop.threshold != 0, [&](auto drop) {
-            hipLaunchKernelGGL((norm_forward_walk_kernel<double, 256 / kSetRows, decltype(drop)::value, true>), grid, dim3(256), 0, s, a);
-        });
+        with_set_shape(a.cols, [&](auto tpr) { with_flag(a.drop.threshold != 0, [&](auto drop) {
+            constexpr int TPR = decltype(tpr)::value, kRows = 256 / TPR;
+            hipLaunchKernelGGL((norm_forward_walk_kernel<double, TPR, decltype(drop)::value, true>),
+                               dim3((unsigned)std::min((a.rows + kRows - 1) / kRows, kMaxBlocks)), dim3(256), 0, s, a);
+        }); });
         return hipGetLastError();
     }
     with_type(type, [&](auto t) {
@@ -1065,11 +1070,12 @@ hipError_t launch_norm_backward(LayerType type, const NormArgs& args, hipStream_
     NormArgs a = args;
     a.inv_cols = 1.0 / (double)a.cols;
     if (a.sets.count) {
-        const SplitShape sh = split_shape(a, 256 / kSetRows);
-        const dim3 grid((unsigned)(sh.row_blocks + std::min(sh.col_tiles * sh.segs, kMaxBlocks)));
-        with_flag(a.drop.threshold != 0, [&](auto drop) {
-            hipLaunchKernelGGL((norm_backward_split_kernel<double, 256 / kSetRows, decltype(drop)::value, true>), grid, dim3(256), 0, s, a, sh);
-        });
+        with_set_shape(a.cols, [&](auto tpr) { with_flag(a.drop.threshold != 0, [&](auto drop) {
+            constexpr int TPR = decltype(tpr)::value;
+            const SplitShape sh = split_shape(a, TPR);
+            hipLaunchKernelGGL((norm_backward_split_kernel<double, TPR, decltype(drop)::value, true>),
+                               dim3((unsigned)(sh.row_blocks + std::min(sh.col_tiles * sh.segs, kMaxBlocks))), dim3(256), 0, s, a, sh);
+        }); });
         return hipGetLastError();
     }
     with_type(type, [&](auto t) {
