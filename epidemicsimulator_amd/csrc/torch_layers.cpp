@@ -5,6 +5,7 @@
 //
 // The entry points are handed over as addresses, so this module needs no libepi.so of its own beside the one that is
 // loaded already.
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -72,6 +73,7 @@ void check_like(const char* name, const Tensor& t, const Tensor& x) {
 // A tensor whose rows (the last dimension) are evenly spaced, and their distance: t itself, or a copy.
 std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
     const int64_t cols = t.size(-1);
+    if (t.is_neg()) return {t.resolve_neg().contiguous(), cols};   // a view whose values are the memory's, negated
     if (t.is_contiguous()) return {t, cols};
     if (cols == 1 || t.stride(-1) == 1) {
         // distance of the last leading dimension of more than one index; the others have to follow from it
@@ -93,7 +95,7 @@ Tensor vector_of(const char* name, const Tensor& w, const Tensor& x) {
     if (!w.defined()) return w;
     check_like(name, w, x);
     if (w.dim() != 1 || w.size(0) != x.size(-1)) refuse(std::string(name) + " has the shape " + str(w.sizes()) + " for " + str(x.size(-1)) + " columns");
-    return w.contiguous();
+    return (w.is_neg() ? w.resolve_neg() : w).contiguous();
 }
 
 // What a call drops with; `offset_dev` may be undefined.
@@ -224,10 +226,25 @@ struct NormNode : torch::autograd::Node {
     std::string name() const override { return "EpiLayerNormBackward"; }
 };
 
+// A leaf that an eager graph still holds collects its gradient on that graph's stream.  A backward pass captured into a
+// HIP graph meanwhile would wait across the two streams, which is no part of a capture and ends the process: refused
+// while the forward pass is being captured.
+void check_capture(std::initializer_list<Tensor> leaves, const Tensor& x) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto here = c10::hip::getCurrentHIPStream(x.get_device()).id();
+    for (const Tensor& t : leaves) {
+        if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+        const auto collects = torch::autograd::impl::try_get_grad_accumulator(t);
+        if (collects && collects->stream() && collects->stream()->id() != here)
+            refuse("an eager graph of the same leaf is alive: drop its outputs before capturing, or capture layer_norm_forward and layer_norm_backward");
+    }
+}
+
 template <class N>
 std::shared_ptr<N> new_node() { return std::shared_ptr<N>(new N(), torch::autograd::deleteNode); }
 
 Tensor record_dropout(const Tensor& x, const Drop& drop) {
+    check_capture({x}, x);
     Tensor y;
     {
         at::AutoGradMode off(false);
@@ -242,6 +259,7 @@ Tensor record_dropout(const Tensor& x, const Drop& drop) {
     return y;
 }
 Tensor record_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps, const Drop& drop) {
+    check_capture({x, w, b}, x);
     std::pair<Tensor, Tensor> r;
     {
         at::AutoGradMode off(false);

@@ -5,7 +5,8 @@ They are what a Q-network is regularised with that replays its buffer many times
 ReLU); the learners of `Agents` run the same kernels inside their networks (`Agents.regularise`).  All arithmetic is in
 libepi.so (epi_dropout, epi_layer_norm_forward, epi_layer_norm_backward of include/epi.h); a tensor that is not on a GPU
 is refused.  Work is enqueued on torch's current stream of the tensor's device, and every array, the workspaces among
-them, is one of torch's, so calls can be captured into a graph.  Leading dimensions are rows, the last one the columns;
+them, is one of torch's, so calls can be captured into a graph (a number as dropout offset is captured with it: every
+replay then drops the same units; a tensor's value is read by every replay).  Leading dimensions are rows, the last one the columns;
 tensors whose rows are evenly spaced are read where they are, others are copied first.
 """
 import ctypes as C
@@ -50,7 +51,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5, dropout: float = 0.0, seed: int = 0, offset: Offset = 0) -> torch.Tensor:
     """(h - mean h) / sqrt(mean (h - mean h)^2 + eps) * weight + bias over the last dimension, with h = x, or
     h = dropout(x, dropout, seed, offset) in the same pass; differentiable in x, weight and bias.  weight and bias hold
-    x's type; sums are taken in float32 (float64 for float64) and y is rounded once."""
+    x's type; sums are taken in float32 (float64 for float64) and y is rounded once.  Captured into a graph with its
+    backward pass while an eager graph of the same leaves is alive, the call is refused."""
     return _layers.layer_norm(x, weight, bias, eps, dropout, seed, offset)
 
 

@@ -352,6 +352,24 @@ def test_more_than_two_to_the_31_elements(L, cols):
     assert not dx[:-6].any()
 
 
+def test_more_chunks_than_one_launch_holds(L):
+    """Over 2^31 chunks of eight: the rows behind the first launch draw and land where they belong."""
+    rows, cols = (1 << 30) + 4099, 9
+    x = torch.randn(1, cols, device="cuda").to(torch.bfloat16).expand(rows, cols)
+    y = L.dropout(x, 0.5, 77, 3)
+    for start in (0, (1 << 30) - 6, rows - 6):
+        f = R.factors(6, cols, 0.5, 77, 3, first_row=start)
+        assert np.array_equal(host(y[start:start + 6]), R.apply_factors(host(x[:6]), f))
+
+
+def test_negated_views(L):
+    z = torch.conj(torch.complex(torch.randn(5, 20), torch.randn(5, 20)).cuda())
+    x = z.imag
+    assert x.is_neg()
+    assert torch.equal(L.dropout(x, 0.5, 1), L.dropout(x.resolve_neg().contiguous(), 0.5, 1))
+    assert torch.equal(L.layer_norm(x, x[0], x[1]), L.layer_norm(x.clone(), x[0].clone(), x[1].clone()))
+
+
 # ---- repeatability, streams, graphs ------------------------------------------------------------------------
 @pytest.mark.parametrize("rows, cols", [(500, 128), (30000, 200), (4000, 4096)])
 def test_the_same_call_gives_the_same_bits(L, rows, cols):
@@ -443,6 +461,35 @@ def test_a_training_step_captured_with_autograd(L):
             assert torch.equal(p, q)
 
 
+def test_capture_beside_an_eager_graph_of_the_leaves_is_refused(L):
+    from epidemicsimulator_amd import _capi
+    x, w, b, dy = make(200, 128, torch.float32, 72)
+    w.requires_grad_(True)
+    alive = L.layer_norm(x, w, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m, r = L.layer_norm_forward(x, w, b)[1:]
+        L.layer_norm_backward(dy, x, w, m, r)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(_capi.EpiError, match="eager graph"):
+            L.layer_norm(x, w, b)
+        y, m, r = L.layer_norm_forward(x, w, b)              # the way round it
+        grads = L.layer_norm_backward(dy, x, w, m, r)
+    for _ in range(3):
+        with torch.no_grad():
+            x.add_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = L.layer_norm_forward(x, w, b)
+        assert torch.equal(y, want[0])
+        for p, q in zip(grads, L.layer_norm_backward(dy, x, w, *want[1:])):
+            assert torch.equal(p, q)
+    del alive
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------
 def test_refusals_of_tensors(L):
     from epidemicsimulator_amd import _capi
@@ -458,6 +505,10 @@ def test_refusals_of_tensors(L):
     for f in wrong:
         with pytest.raises(_capi.EpiError):
             f()
+    d = _capi.LayerDesc(rows=4, cols=8, x_stride=8, y_stride=8, dtype=1, device=torch.cuda.device_count())
+    import ctypes as C
+    assert _capi.lib().epi_dropout(C.byref(d), x.data_ptr(), y.data_ptr(), None) == _capi.EPI_ERR_BAD_ARGUMENT   # no such device
+    assert torch.cuda.current_device() == 0
     with pytest.raises(RuntimeError):   # no second derivatives
         t = x.clone().requires_grad_(True)
         g, = torch.autograd.grad(L.layer_norm(t).square().sum(), t, create_graph=True)
