@@ -909,8 +909,9 @@ auto with_flag(bool on, F f) {
 }
 
 // Threads of a row and chunks of a thread for rows that are held in registers: calls f(threads, chunks) and returns
-// true, or returns false for rows that are too narrow or too wide.  Up to 1,024 columns a row stays in a wave: no
-// barrier.  Beyond, the smallest workgroup with one chunk a thread, while there is one: at 16,384 x 4,096 bfloat16 the
+// true, or returns false for rows that are too narrow or too wide.  Up to 1,024 columns (forward 1,536) a row stays in
+// a wave: no barrier (60,000 x 1,500 bfloat16 with dropout forward: 85 us with 64 x 3, 111 with 256 x 1; backward, where
+// the sums take the registers, 180 and 152).  Beyond, the smallest workgroup with one chunk a thread, while there is one: at 16,384 x 4,096 bfloat16 the
 // backward pass takes 91 us with 512 x 1, 122 with 256 x 2 and 145 with 128 x 4, because the next row's registers
 // then fit beside the sums; the forward pass, which has no sums, does not care (47.2, 50.3, 53.0).  Backward rows that
 // need more registers than a wave has are left to the split kernels, which read x and dy twice: 4,000 x 24,000
@@ -926,6 +927,7 @@ bool with_row_shape(int64_t cols, F f) {
     else if (cols <= 256) f(int_c<32>{}, int_c<1>{});
     else if (cols <= 512) f(int_c<64>{}, int_c<1>{});
     else if (cols <= 1024) f(int_c<64>{}, int_c<2>{});
+    else if (FORWARD && cols <= 1536) f(int_c<64>{}, int_c<3>{});
     else if (cols <= 2048) f(int_c<256>{}, int_c<1>{});
     else if (cols <= 4096) f(int_c<512>{}, int_c<1>{});
     else if (cols <= 8192) f(int_c<FORWARD ? 512 : 1024>{}, int_c<FORWARD ? 2 : 1>{});
@@ -950,12 +952,14 @@ int64_t forward_blocks(int64_t rows) {
 // Workgroups of the backward pass.  Each leaves a partial row of both gradients, so here fewer are better until the
 // device is no longer full: a row in a wave, 512 (24,576 x 128 float: 12.0 us, 13.0 with 256, 14.0 with 1,024), and 768
 // where rows are many (819,200 x 128 bfloat16: 122.8 us, 127.6 with 512, 127.0 with 1,024); a row in a workgroup, what
-// fills the device four waves deep.
+// fills the device four waves deep, and half of it for a few thousand rows of one workgroup of 256 threads each (3,000 x
+// 2,000 bfloat16: 21.3 us, 27.5 with 1,024; 9,001 x 1,500 half: 33.3 with 512, 31.3).
 template <int TPR>
 int64_t backward_blocks(int64_t rows) {
     constexpr int kRows = norm_threads(TPR) / TPR;
-    const int64_t most = TPR > 64 ? (int64_t)1024 * 256 / norm_threads(TPR)
-                                  : std::min<int64_t>(768, std::max<int64_t>(rows / (kRows * 16), 512));
+    const int64_t most = TPR <= 64    ? std::min<int64_t>(768, std::max<int64_t>(rows / (kRows * 16), 512))
+                         : TPR == 256 ? (rows < 8192 ? 512 : 1024)
+                                      : (int64_t)1024 * 256 / norm_threads(TPR);
     return std::min((rows + kRows - 1) / kRows, most);
 }
 // Up to so many rows the split kernel does it all in one launch (1,536 x 128 float: 9.6 us there, 7.1 here).
