@@ -223,6 +223,18 @@ __device__ inline void drop_chunk(const Keep& keep, A scale, A (&v)[kChunk]) {
     for (int k = 0; k < kChunk; ++k) v[k] = keep(k) ? v[k] * scale : (A)0;
 }
 
+__device__ inline uint32_t pack(const Keep& keep) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) bits |= keep(k) ? 1u << k : 0u;
+    return bits;
+}
+template <class A>
+__device__ inline void drop_bits(uint32_t bits, A scale, A (&v)[kChunk]) {
+#pragma unroll
+    for (int k = 0; k < kChunk; ++k) v[k] = (bits >> k & 1) ? v[k] * scale : (A)0;
+}
+
 // ---- sums over the threads of a row ---------------------------------------------------------------
 // One step of a sum over 2 * D lanes whose halves hold a value each: every lane adds the other half's value.  Steps
 // within 16 lanes are data-parallel moves of the vector unit, the two beyond swap rows of 16 or 32 lanes; nothing goes
@@ -715,16 +727,20 @@ __global__ __launch_bounds__(256) void norm_backward_split_kernel(NormArgs a, Sp
 // loaded: u and g are formed twice, before and after the row's two means, which is cheaper than the registers of a
 // widened copy.  Bound by memory while a wave's registers hold a row: 819,200 x 128 bfloat16 take 122 us with the
 // reduction (5.1 TB/s over x, dy and dx), 16,384 x 4,096 bfloat16 91 us (4.4 TB/s: 5 of them are the reduction of 512
-// partial rows); beyond 8,192 columns by the registers (6,000 x 16,000 bfloat16: 171 us, 3.4 TB/s).
+// partial rows); beyond 8,192 columns by what a workgroup of 1,024 threads can hold (6,000 x 16,000 bfloat16: 158 us,
+// 3.6 TB/s; with dw's sums in registers 171; with dropout, where x and dy are fetched again for the second half, 176 --
+// held they take 207 for 16-bit types, but 155 against 164 for float at 4,000 x 12,000).
 template <class T, int TPR, int NV, bool DROP>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormArgs a) {
     using A = wide_t<T>;
     constexpr int kRows = norm_threads(TPR) / TPR;
-    constexpr bool kKeep = NV * sizeof(T) <= 8;      // registers for x and dy of the row
+    constexpr bool kWide = TPR == 1024 && NV > 1;    // dw's sums in LDS, the dropped units as bits
+    constexpr bool kKeep = NV * sizeof(T) <= 8 && !(kWide && DROP && sizeof(T) == 2);   // registers for x and dy of the row
     constexpr bool kAhead = NV * sizeof(T) <= 4;     // and of the next row
     constexpr bool kHold = NV == 1 && sizeof(T) < 8; // registers for the weights
     constexpr int kCols = TPR * NV * kChunk;
     __shared__ A lds[TPR > 64 ? kRowLds<TPR, 2> : 4 * kCols];
+    __shared__ A wide[kWide ? kCols : 1];             // [chunk of a thread][half][thread][4]
     int flip = 0;
     const int t = threadIdx.x % TPR, cols = (int)a.cols;
     int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
@@ -733,11 +749,16 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
     const A inv = (A)a.inv_cols, scale = (A)a.drop.scale;
     uint32_t off[2] = {0, 0};
     if constexpr (DROP) drop_offset(a.drop, off);
-    A gw[NV][kChunk], gb[NV][kChunk], hg[kChunk];
+    A gw[kWide ? 1 : NV][kChunk], gb[NV][kChunk], hg[kChunk];
+    auto in_lds = [&](int v, int k) -> A& { return wide[((v * 2 + k / 4) * TPR + t) * 4 + k % 4]; };
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int k = 0; k < kChunk; ++k) gw[v][k] = gb[v][k] = 0;
+        for (int k = 0; k < kChunk; ++k) {
+            gb[v][k] = 0;
+            if constexpr (kWide) in_lds(v, k) = 0;
+            else gw[v][k] = 0;
+        }
     auto gains = [&](int v, A (&g)[kChunk]) {
 #pragma unroll
         for (int k = 0; k < kChunk; ++k) g[k] = 1;
@@ -764,7 +785,8 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
         if constexpr (kAhead) {
             if (next < a.rows) fetch(next, nx, nd, nm, nr);
         }
-        Keep keep[NV];
+        Keep keep[kWide ? 1 : NV];
+        uint32_t bits[NV];
         A s[2] = {0, 0};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -775,14 +797,21 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
             widen_chunk(rd[kKeep ? v : 0], g);
             if constexpr (!kHold) gains(v, w);
             if constexpr (DROP) {
-                keep[v] = keep_at(a.drop, off, p, (uint32_t)row);
-                drop_chunk(keep[v], scale, u);
+                Keep& kp = keep[kWide ? 0 : v];
+                kp = keep_at(a.drop, off, p, (uint32_t)row);
+                drop_chunk(kp, scale, u);
+                if constexpr (kWide) bits[v] = pack(kp);
             }
             clear_head(p.skip, g);
+            if constexpr (kWide) {
+#pragma unroll
+                for (int k = 0; k < kChunk; ++k) gw[0][k] = in_lds(v, k);
+            }
 #pragma unroll
             for (int k = 0; k < kChunk; ++k) {
                 u[k] = (u[k] - m) * r;
-                gw[v][k] += g[k] * u[k];
+                gw[kWide ? 0 : v][k] += g[k] * u[k];
+                if constexpr (kWide) in_lds(v, k) = gw[0][k];
                 gb[v][k] += g[k];
                 g[k] *= kHold ? hg[k] : w[k];
                 s[0] += g[k];
@@ -804,14 +833,14 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
                 widen_chunk(rx[kKeep ? v : 0], u);
                 widen_chunk(rd[kKeep ? v : 0], g);
                 if constexpr (!kHold) gains(v, w);
-                if constexpr (DROP) drop_chunk(keep[v], scale, u);
+                if constexpr (DROP) { if constexpr (kWide) drop_bits(bits[v], scale, u); else drop_chunk(keep[kWide ? 0 : v], scale, u); }
 #pragma unroll
                 for (int k = 0; k < kChunk; ++k) {
                     u[k] = (u[k] - m) * r;
                     g[k] *= kHold ? hg[k] : w[k];
                     g[k] = ((g[k] - c1) - u[k] * c2) * r;
                 }
-                if constexpr (DROP) drop_chunk(keep[v], scale, g);
+                if constexpr (DROP) { if constexpr (kWide) drop_bits(bits[v], scale, g); else drop_chunk(keep[kWide ? 0 : v], scale, g); }
                 Raw<T> o;
                 narrow_chunk<T>(g, o);
                 put_part<T, kChunk>(dx + p.col, o.w);
@@ -834,7 +863,11 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
             const Spot p = spot_of(cols, t + v * TPR);
 #pragma unroll
             for (int k = 0; k < kChunk; ++k)
-                if (k >= p.skip) { part[p.col + k] = gw[v][k]; part[cols + p.col + k] = gb[v][k]; }
+                if (k >= p.skip) {
+                    if constexpr (kWide) part[p.col + k] = in_lds(v, k);
+                    else part[p.col + k] = gw[v][k];
+                    part[cols + p.col + k] = gb[v][k];
+                }
         }
     } else {
 #pragma unroll
@@ -845,7 +878,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
                 const Spot p = spot_of(cols, t + v * TPR);
 #pragma unroll
                 for (int k = 0; k < kChunk; ++k) {
-                    A z = which ? gb[v][k] : gw[v][k];
+                    A z = which ? gb[v][k] : gw[kWide ? 0 : v][k];
 #pragma unroll
                     for (int n = TPR; n < 64; n <<= 1) z += __shfl_xor(z, n, 64);
                     if ((threadIdx.x & 63) < TPR && k >= p.skip) lds[(threadIdx.x >> 6) * kCols + p.col + k] = z;
@@ -913,12 +946,12 @@ auto with_flag(bool on, F f) {
 // a wave: no barrier (60,000 x 1,500 bfloat16 with dropout forward: 85 us with 64 x 3, 111 with 256 x 1; backward, where
 // the sums take the registers, 180 and 152).  Beyond, the smallest workgroup with one chunk a thread, while there is one: at 16,384 x 4,096 bfloat16 the
 // backward pass takes 91 us with 512 x 1, 122 with 256 x 2 and 145 with 128 x 4, because the next row's registers
-// then fit beside the sums; the forward pass, which has no sums, does not care (47.2, 50.3, 53.0).  Backward rows that
-// need more registers than a wave has are left to the split kernels, which read x and dy twice: 4,000 x 24,000
-// bfloat16 take 262 us there and 296 with 1,024 x 3, 1,500 x 12,000 double 165 and 299, but 6,000 x 16,000 bfloat16 261
-// and 171 with 1,024 x 2, 3,000 x 8,000 double 237 and 192 with 1,024 x 1.
+// then fit beside the sums; the forward pass, which has no sums, does not care (47.2, 50.3, 53.0).  Backward rows of
+// more than one chunk a thread keep dw's sums in LDS; where registers still run out, the split kernels take them,
+// which read x and dy twice: 4,000 x 24,000 bfloat16 take 186 us with 1,024 x 3 and 262 split, but 312 and 263 with
+// dropout; 2,500 x 32,000 300 and 226; 1,500 x 12,000 double 299 and 165.
 template <int N> using int_c = std::integral_constant<int, N>;
-template <class T, bool FORWARD, class F>
+template <class T, bool FORWARD, bool DROP, class F>
 bool with_row_shape(int64_t cols, F f) {
     if (cols < kChunk) return false;
     if (cols <= 32) f(int_c<4>{}, int_c<1>{});
@@ -933,8 +966,9 @@ bool with_row_shape(int64_t cols, F f) {
     else if (cols <= 8192) f(int_c<FORWARD ? 512 : 1024>{}, int_c<FORWARD ? 2 : 1>{});
     else if constexpr (!FORWARD && sizeof(T) == 8) return false;
     else if (cols <= 16384) f(int_c<1024>{}, int_c<2>{});
-    else if constexpr (!FORWARD) return false;
+    else if constexpr (!FORWARD && DROP) return false;
     else if (cols <= 24576) f(int_c<1024>{}, int_c<3>{});
+    else if constexpr (!FORWARD) return false;
     else if (cols <= 32768) f(int_c<1024>{}, int_c<4>{});
     else return false;
     return true;
@@ -1042,7 +1076,7 @@ hipError_t launch_norm_forward(LayerType type, const NormArgs& args, hipStream_t
         using T = decltype(t);
         with_flag(a.drop.threshold != 0, [&](auto drop) {
             constexpr bool D = decltype(drop)::value;
-            const bool held = with_row_shape<T, true>(a.cols, [&](auto tpr, auto nv) {
+            const bool held = with_row_shape<T, true, D>(a.cols, [&](auto tpr, auto nv) {
                 constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
                 hipLaunchKernelGGL((norm_forward_kernel<T, TPR, NV, D>), dim3((unsigned)forward_blocks<TPR>(a.rows)), dim3(norm_threads(TPR)), 0, s, a);
             });
@@ -1056,12 +1090,14 @@ hipError_t launch_norm_forward(LayerType type, const NormArgs& args, hipStream_t
     return hipGetLastError();
 }
 
-size_t norm_backward_workspace(LayerType type, int64_t rows, int64_t cols) {
+size_t norm_backward_workspace(LayerType type, int64_t rows, int64_t cols, bool drop) {
     return with_type(type, [&](auto t) -> size_t {
         using T = decltype(t);
         int64_t parts = 0;
         if (rows > kSplitRows)
-            with_row_shape<T, false>(cols, [&](auto tpr, auto) { parts = backward_blocks<decltype(tpr)::value>(rows); });
+            with_flag(drop, [&](auto on) {
+                with_row_shape<T, false, decltype(on)::value>(cols, [&](auto tpr, auto) { parts = backward_blocks<decltype(tpr)::value>(rows); });
+            });
         if (!parts) {
             const int64_t segs = (rows + kSegRows - 1) / kSegRows;
             parts = segs > 1 ? segs : 0;
@@ -1096,7 +1132,7 @@ hipError_t launch_norm_backward(LayerType type, const NormArgs& args, hipStream_
         with_flag(a.drop.threshold != 0, [&](auto drop) {
             constexpr bool D = decltype(drop)::value;
             if (a.rows > kSplitRows)
-                with_row_shape<T, false>(a.cols, [&](auto tpr, auto nv) {
+                with_row_shape<T, false, D>(a.cols, [&](auto tpr, auto nv) {
                     constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
                     NormArgs b = a;
                     if (!vectors) b.workspace = nullptr;
@@ -1233,7 +1269,7 @@ EPI_API int32_t epi_layer_norm_backward_workspace(const epi_layer_desc* d, size_
     Extent e{};
     if (int32_t rc = check_desc("layer_norm_backward_workspace", d, &e)) return rc;
     if (!bytes) return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_backward_workspace: null argument");
-    *bytes = norm_backward_workspace((LayerType)d->dtype, d->rows, d->cols);
+    *bytes = norm_backward_workspace((LayerType)d->dtype, d->rows, d->cols, make_drop(d->dropout, 0, 0, nullptr).threshold != 0);
     return EPI_OK;
 }
 
@@ -1256,7 +1292,7 @@ EPI_API int32_t epi_layer_norm_backward(const epi_layer_desc* d, const void* x, 
     for (const auto& v : vectors)
         if (int32_t rc = check_vector(who, v.name, v.p, v.size)) return rc;
     size_t need = 0;
-    if (dweight || dbias) need = norm_backward_workspace((LayerType)d->dtype, d->rows, d->cols);
+    if (dweight || dbias) need = norm_backward_workspace((LayerType)d->dtype, d->rows, d->cols, make_drop(d->dropout, 0, 0, nullptr).threshold != 0);
     if (need && (!workspace || workspace_bytes < need))
         return fail(EPI_ERR_BAD_ARGUMENT, "layer_norm_backward: a workspace of %zu bytes is needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     const struct { const void* p; int64_t n; } in[] = {

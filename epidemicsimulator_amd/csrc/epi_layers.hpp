@@ -49,7 +49,7 @@ enum LayerType { kF64 = 0, kF32 = 1, kBF16 = 2, kF16 = 3 };
 hipError_t launch_dropout(LayerType type, int64_t rows, int64_t cols, int64_t x_stride, int64_t y_stride, const void* x,
                           void* y, const DropArgs& drop, hipStream_t s);
 hipError_t launch_norm_forward(LayerType type, const NormArgs& a, hipStream_t s);
-size_t norm_backward_workspace(LayerType type, int64_t rows, int64_t cols);
+size_t norm_backward_workspace(LayerType type, int64_t rows, int64_t cols, bool drop);
 hipError_t launch_norm_backward(LayerType type, const NormArgs& a, hipStream_t s);
 
 }  // namespace epi

@@ -462,7 +462,7 @@ int32_t epi_dropout(const epi_layer_desc *d, const void *x, void *y, void *strea
  * everything between load and store are in the type of mean; y is rounded once.  y may be x. */
 int32_t epi_layer_norm_forward(const epi_layer_desc *d, const void *x, const void *weight, const void *bias, void *y,
                                void *mean, void *rstd, void *stream);
-/* Bytes of workspace that epi_layer_norm_backward needs for a descriptor's dtype, rows and cols (may be 0). */
+/* Bytes of workspace that epi_layer_norm_backward needs for a descriptor's dtype, rows, cols and dropout (may be 0). */
 int32_t epi_layer_norm_backward_workspace(const epi_layer_desc *d, size_t *bytes);
 /* dx[rows][cols], dweight[cols] and dbias[cols] (each may be NULL) from x, dy, weight (NULL = ones) and the mean and
  * rstd of the forward pass, with the same dropout, seed and offset.  Sums over the rows are taken in a fixed order in

@@ -128,6 +128,14 @@ def test_norm_many_wide_rows(L, rows, cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES.values()), ids=list(TYPES))
+@pytest.mark.parametrize("rows, cols", [(1100, 1536), (1100, 1537), (1050, 8193), (1050, 12001), (1030, 16384), (1030, 16392), (1026, 20003),
+                                        (1026, 24576), (1026, 24585), (1026, 7)])
+def test_norm_backward_shapes_with_and_without_dropout(L, rows, cols, dtype):
+    both_ways(L, dtype, rows, cols, 0.0)
+    both_ways(L, dtype, rows, cols, 0.3)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES.values()), ids=list(TYPES))
 def test_norm_far_means_and_small_spreads(L, dtype):
     """Means of 1,000 spreads (64 in 8 bits of mantissa), and rows of one value each: the spread is then zero."""
     both_ways(L, dtype, 9, 300, 0.0, mean=64.0 if dtype == torch.bfloat16 else 1000.0)
