@@ -223,6 +223,7 @@ __device__ inline void drop_chunk(const Keep& keep, A scale, A (&v)[kChunk]) {
     for (int k = 0; k < kChunk; ++k) v[k] = keep(k) ? v[k] * scale : (A)0;
 }
 
+// The same as one bit a unit.
 __device__ inline uint32_t pack(const Keep& keep) {
     uint32_t bits = 0;
 #pragma unroll
@@ -787,6 +788,10 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
         }
         Keep keep[kWide ? 1 : NV];
         uint32_t bits[NV];
+        auto drop_again = [&](int v, A (&c)[kChunk]) {
+            if constexpr (DROP && kWide) drop_bits(bits[v], scale, c);
+            else if constexpr (DROP) drop_chunk(keep[v], scale, c);
+        };
         A s[2] = {0, 0};
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -833,14 +838,14 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
                 widen_chunk(rx[kKeep ? v : 0], u);
                 widen_chunk(rd[kKeep ? v : 0], g);
                 if constexpr (!kHold) gains(v, w);
-                if constexpr (DROP) { if constexpr (kWide) drop_bits(bits[v], scale, u); else drop_chunk(keep[kWide ? 0 : v], scale, u); }
+                drop_again(v, u);
 #pragma unroll
                 for (int k = 0; k < kChunk; ++k) {
                     u[k] = (u[k] - m) * r;
                     g[k] *= kHold ? hg[k] : w[k];
                     g[k] = ((g[k] - c1) - u[k] * c2) * r;
                 }
-                if constexpr (DROP) { if constexpr (kWide) drop_bits(bits[v], scale, g); else drop_chunk(keep[kWide ? 0 : v], scale, g); }
+                drop_again(v, g);
                 Raw<T> o;
                 narrow_chunk<T>(g, o);
                 put_part<T, kChunk>(dx + p.col, o.w);
@@ -944,12 +949,12 @@ auto with_flag(bool on, F f) {
 // Threads of a row and chunks of a thread for rows that are held in registers: calls f(threads, chunks) and returns
 // true, or returns false for rows that are too narrow or too wide.  Up to 1,024 columns (forward 1,536) a row stays in
 // a wave: no barrier (60,000 x 1,500 bfloat16 with dropout forward: 85 us with 64 x 3, 111 with 256 x 1; backward, where
-// the sums take the registers, 180 and 152).  Beyond, the smallest workgroup with one chunk a thread, while there is one: at 16,384 x 4,096 bfloat16 the
-// backward pass takes 91 us with 512 x 1, 122 with 256 x 2 and 145 with 128 x 4, because the next row's registers
-// then fit beside the sums; the forward pass, which has no sums, does not care (47.2, 50.3, 53.0).  Backward rows of
-// more than one chunk a thread keep dw's sums in LDS; where registers still run out, the split kernels take them,
-// which read x and dy twice: 4,000 x 24,000 bfloat16 take 186 us with 1,024 x 3 and 262 split, but 312 and 263 with
-// dropout; 2,500 x 32,000 300 and 226; 1,500 x 12,000 double 299 and 165.
+// the sums take the registers, 180 and 152).  Beyond, the smallest workgroup with one chunk a thread, while there is
+// one: at 16,384 x 4,096 bfloat16 the backward pass takes 91 us with 512 x 1, 122 with 256 x 2 and 145 with 128 x 4,
+// because the next row's registers then fit beside the sums; the forward pass, which has no sums, does not care (47.2,
+// 50.3, 53.0).  Backward rows of more than one chunk a thread keep dw's sums in LDS; where registers still run out, the
+// split kernels take them, which read x and dy twice: 4,000 x 24,000 bfloat16 take 186 us with 1,024 x 3 and 262 split,
+// but 312 and 263 with dropout; 2,500 x 32,000 300 and 226; 1,500 x 12,000 double 299 and 165.
 template <int N> using int_c = std::integral_constant<int, N>;
 template <class T, bool FORWARD, bool DROP, class F>
 bool with_row_shape(int64_t cols, F f) {
@@ -960,7 +965,7 @@ bool with_row_shape(int64_t cols, F f) {
     else if (cols <= 256) f(int_c<32>{}, int_c<1>{});
     else if (cols <= 512) f(int_c<64>{}, int_c<1>{});
     else if (cols <= 1024) f(int_c<64>{}, int_c<2>{});
-    else if (FORWARD && cols <= 1536) f(int_c<64>{}, int_c<3>{});
+    else if (FORWARD && cols <= 1536) f(int_c<64>{}, int_c<FORWARD ? 3 : 2>{});
     else if (cols <= 2048) f(int_c<256>{}, int_c<1>{});
     else if (cols <= 4096) f(int_c<512>{}, int_c<1>{});
     else if (cols <= 8192) f(int_c<FORWARD ? 512 : 1024>{}, int_c<FORWARD ? 2 : 1>{});
