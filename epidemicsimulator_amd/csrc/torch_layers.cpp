@@ -1,6 +1,6 @@
 // torch binding of the layer operators (epi_dropout, epi_layer_norm_* of include/epi.h): argument checks, the tensors a
 // call needs, and the autograd nodes.  In C++ because a training step of a small layer is all host time: 512 x 128
-// doubles, forward and gradients through torch.autograd.grad, take 64 us this way and 118 with nodes written in
+// doubles, forward and gradients through torch.autograd.grad, take 60 us this way and 118 with nodes written in
 // Python, whose backward pass waits for the interpreter in another thread; the kernels of both together take 12.
 //
 // The entry points are handed over as addresses, so this module needs no libepi.so of its own beside the one that is

@@ -244,6 +244,32 @@ def test_gradients_against_differences(L, rows, cols, p):
     assert torch.autograd.gradcheck(lambda a: L.dropout(a, p, 3, 1), leaves[:1])
 
 
+def test_the_graph_keeps_autograds_rules(L):
+    """Backward twice only where the graph is retained; inputs changed in between are noticed; a weight that is the bias
+    too, or expanded from one number, collects both or all of its gradients."""
+    x, w, b, dy = make(50, 40, torch.float64, 22)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = L.layer_norm(x, w, b)
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    for p, q in zip(first, torch.autograd.grad(y, leaves, dy)):
+        assert torch.equal(p, q)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, leaves, dy)
+    y = L.layer_norm(x, w, b)
+    with torch.no_grad():
+        x.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        torch.autograd.grad(y, leaves, dy)
+    dw, db = torch.autograd.grad(L.layer_norm(x, w, b), (w, b), dy)
+    both, = torch.autograd.grad(L.layer_norm(x, w, w), w, dy)
+    assert torch.equal(both, dw + db)
+    one = torch.ones(1, device="cuda", dtype=torch.float64, requires_grad=True)
+    g, = torch.autograd.grad(L.layer_norm(x, one.expand(40), b), one, dy)
+    assert torch.allclose(g, dw.sum().reshape(1), rtol=1e-12, atol=1e-12)
+    with torch.inference_mode():
+        assert torch.equal(L.layer_norm(x.clone(), w.clone(), b.clone()), L.layer_norm_forward(x, w, b)[0])
+
+
 # ---- layouts -------------------------------------------------------------------------------------------
 def test_strided_expanded_and_transposed_rows(L):
     wide, w, b, dyw = make(40, 300, torch.float32, 31)

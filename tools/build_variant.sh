@@ -9,7 +9,7 @@ mkdir -p "$tmp/epidemicsimulator_amd" "$root/build"
 cp -r "$root/include" "$tmp/include"
 cp -r "$root/epidemicsimulator_amd/csrc" "$tmp/epidemicsimulator_amd/csrc"
 rm -f "$tmp"/epidemicsimulator_amd/csrc/*.o
-make -s -C "$tmp/epidemicsimulator_amd/csrc" EXTRA="$*" >/dev/null
+make -s -C "$tmp/epidemicsimulator_amd/csrc" EXTRA="$*" ../libepi.so >/dev/null
 cp "$tmp/epidemicsimulator_amd/libepi.so" "$root/build/libepi_$name.so"
 rm -rf "$tmp"
 echo "build/libepi_$name.so"
