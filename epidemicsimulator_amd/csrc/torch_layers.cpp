@@ -59,6 +59,7 @@ int32_t dtype_of(const Tensor& t) {
 }
 
 void check_x(const char* name, const Tensor& x) {
+    if (!lib.dropout) refuse("import epidemicsimulator_amd.layers: this module is a part of it");
     if (!x.defined()) refuse(std::string(name) + " is missing");
     if (!x.is_cuda()) refuse(std::string(name) + " is on " + str(x.device()) + ": the operators run on the GPU only");
     if (x.layout() != at::kStrided) refuse(std::string(name) + " is not a strided tensor");
@@ -278,70 +279,168 @@ Tensor record_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps
 }
 
 // ---- what Python calls ------------------------------------------------------------------------------------
+// Plain functions of the interpreter's fast call: a small call is mostly its way here and back.
+
+// Positional and named arguments into slots; `required` of them have to be there.
+template <size_t N>
+bool parse(const char* function, const char* const (&names)[N], size_t required, PyObject* const* args, Py_ssize_t count, PyObject* keywords,
+           PyObject* (&slots)[N]) {
+    for (auto& s : slots) s = nullptr;
+    if (count > (Py_ssize_t)N) {
+        PyErr_Format(PyExc_TypeError, "%s() takes at most %zu arguments, %zd given", function, N, count);
+        return false;
+    }
+    for (Py_ssize_t k = 0; k < count; ++k) slots[k] = args[k];
+    const Py_ssize_t named = keywords ? PyTuple_GET_SIZE(keywords) : 0;
+    for (Py_ssize_t k = 0; k < named; ++k) {
+        PyObject* key = PyTuple_GET_ITEM(keywords, k);
+        size_t at = 0;
+        while (at < N && PyUnicode_CompareWithASCIIString(key, names[at]) != 0) ++at;
+        if (at == N || slots[at]) {
+            PyErr_Format(PyExc_TypeError, at == N ? "%s() has no argument named %R" : "%s() got argument %R twice", function, key);
+            return false;
+        }
+        slots[at] = args[count + k];
+    }
+    for (size_t k = 0; k < required; ++k)
+        if (!slots[k]) {
+            PyErr_Format(PyExc_TypeError, "%s() needs the argument '%s'", function, names[k]);
+            return false;
+        }
+    return true;
+}
+
+double number(PyObject* v, double otherwise) {
+    if (!v) return otherwise;
+    const double d = PyFloat_AsDouble(v);
+    if (d == -1.0 && PyErr_Occurred()) throw python_error();
+    return d;
+}
 // Any integer, taken modulo 2^64.
-int64_t word(const py::handle& v) {
-    const unsigned long long w = PyLong_AsUnsignedLongLongMask(v.ptr());
-    if (PyErr_Occurred()) throw py::error_already_set();
+int64_t word(PyObject* v) {
+    if (!v) return 0;
+    const unsigned long long w = PyLong_AsUnsignedLongLongMask(v);
+    if (w == (unsigned long long)-1 && PyErr_Occurred()) throw python_error();
     return (int64_t)w;
 }
 // Seed and offset as numbers, or the offset as a tensor.
-Drop drop_of(double p, const py::handle& seed, const py::handle& offset) {
+Drop drop_of(PyObject* p, PyObject* seed, PyObject* offset) {
     Drop d;
-    d.p = p;
+    d.p = number(p, 0.0);
     d.seed = word(seed);
-    if (THPVariable_Check(offset.ptr())) d.offset_dev = THPVariable_Unpack(offset.ptr());
+    if (offset && THPVariable_Check(offset)) d.offset_dev = THPVariable_Unpack(offset);
     else d.offset = word(offset);
     return d;
 }
-Tensor tensor_of(const char* name, const py::handle& v, bool optional) {
-    if (optional && v.is_none()) return Tensor();
-    if (!THPVariable_Check(v.ptr())) refuse(std::string(name) + " is not a tensor");
-    return THPVariable_Unpack(v.ptr());
+Tensor tensor_of(const char* name, PyObject* v, bool optional) {
+    if (optional && (!v || v == Py_None)) return Tensor();
+    if (!THPVariable_Check(v)) refuse(std::string(name) + " is not a tensor");
+    return THPVariable_Unpack(v);
 }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
-Tensor dropout(const py::handle& x_, double p, const py::handle& seed, const py::handle& offset) {
-    const Tensor x = tensor_of("x", x_, false);
-    const Drop drop = drop_of(p, seed, offset);
-    py::gil_scoped_release free;
-    check_x("x", x);
-    return at::GradMode::is_enabled() && wants(x) ? record_dropout(x, drop) : run_dropout(x, drop);
+// Runs f; a Failure becomes the package's EpiError, everything else what torch makes of it.
+template <class F>
+PyObject* guarded(F f) {
+    HANDLE_TH_ERRORS
+    try {
+        return f();
+    } catch (const Failure& e) {
+        const py::object type = py::module_::import("epidemicsimulator_amd._capi").attr("EpiError");
+        PyErr_SetObject(type.ptr(), type(e.status, e.what()).ptr());
+        return nullptr;
+    }
+    END_HANDLE_TH_ERRORS
 }
-Tensor layer_norm(const py::handle& x_, const py::handle& w_, const py::handle& b_, double eps, double p, const py::handle& seed, const py::handle& offset) {
-    const Tensor x = tensor_of("x", x_, false), w = tensor_of("weight", w_, true), b = tensor_of("bias", b_, true);
-    const Drop drop = drop_of(p, seed, offset);
-    py::gil_scoped_release free;
-    check_x("x", x);
-    if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) return record_norm(x, w, b, eps, drop);
-    return run_forward(x, w, b, eps, drop, false).first;
+PyObject* triple(const std::tuple<Tensor, Tensor, Tensor>& t) {
+    py::tuple out(3);
+    out[0] = py::reinterpret_steal<py::object>(THPVariable_Wrap(std::get<0>(t)));
+    out[1] = py::reinterpret_steal<py::object>(THPVariable_Wrap(std::get<1>(t)));
+    out[2] = py::reinterpret_steal<py::object>(THPVariable_Wrap(std::get<2>(t)));
+    return out.release().ptr();
 }
-std::tuple<Tensor, Tensor, Tensor> layer_norm_forward(const py::handle& x_, const py::handle& w_, const py::handle& b_, double eps, double p,
-                                                      const py::handle& seed, const py::handle& offset) {
-    const Tensor x = tensor_of("x", x_, false), w = tensor_of("weight", w_, true), b = tensor_of("bias", b_, true);
-    const Drop drop = drop_of(p, seed, offset);
-    py::gil_scoped_release free;
-    at::AutoGradMode off(false);
-    check_x("x", x);
-    const auto [y, stats] = run_forward(x, w, b, eps, drop, true);
-    return {y, stats.select(0, 0), stats.select(0, 1)};
+
+PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t count, PyObject* keywords) {
+    static const char* const names[] = {"x", "p", "seed", "offset"};
+    PyObject* v[4];
+    if (!parse("dropout", names, 3, args, count, keywords, v)) return nullptr;
+    return guarded([&] {
+        const Tensor x = tensor_of("x", v[0], false);
+        const Drop drop = drop_of(v[1], v[2], v[3]);
+        Tensor y;
+        {
+            py::gil_scoped_release free;
+            check_x("x", x);
+            y = at::GradMode::is_enabled() && wants(x) ? record_dropout(x, drop) : run_dropout(x, drop);
+        }
+        return THPVariable_Wrap(std::move(y));
+    });
 }
-std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const py::handle& dy_, const py::handle& x_, const py::handle& w_, const py::handle& mean_,
-                                                       const py::handle& rstd_, double p, const py::handle& seed, const py::handle& offset) {
-    const Tensor dy = tensor_of("dy", dy_, false), x = tensor_of("x", x_, false), w = tensor_of("weight", w_, true);
-    const Tensor mean = tensor_of("mean", mean_, false), rstd = tensor_of("rstd", rstd_, false);
-    const Drop drop = drop_of(p, seed, offset);
-    py::gil_scoped_release free;
-    at::AutoGradMode off(false);
-    check_x("x", x);
-    check_x("dy", dy);
-    check_like("dy", dy, x);
-    if (dy.sizes() != x.sizes()) refuse("dy has the shape " + str(dy.sizes()) + ", x " + str(x.sizes()));
-    const auto wide = x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat;
-    const int64_t rows = x.numel() / x.size(-1);
-    for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"mean", mean}, {"rstd", rstd}})
-        if (t.device() != x.device() || t.scalar_type() != wide || !t.is_contiguous() || t.numel() != rows)
-            refuse(std::string(name) + " is not the forward pass's: " + str(rows) + " numbers of " + str(wide) + " on " + str(x.device()));
-    return run_backward(dy, x, w, mean.data_ptr(), rstd.data_ptr(), drop, true, true, true);
+
+const char* const kNormNames[] = {"x", "weight", "bias", "eps", "dropout", "seed", "offset"};
+
+PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t count, PyObject* keywords) {
+    PyObject* v[7];
+    if (!parse("layer_norm", kNormNames, 1, args, count, keywords, v)) return nullptr;
+    return guarded([&] {
+        const Tensor x = tensor_of("x", v[0], false), w = tensor_of("weight", v[1], true), b = tensor_of("bias", v[2], true);
+        const double eps = number(v[3], 1e-5);
+        const Drop drop = drop_of(v[4], v[5], v[6]);
+        Tensor y;
+        {
+            py::gil_scoped_release free;
+            check_x("x", x);
+            y = at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b)) ? record_norm(x, w, b, eps, drop)
+                                                                                : run_forward(x, w, b, eps, drop, false).first;
+        }
+        return THPVariable_Wrap(std::move(y));
+    });
+}
+
+PyObject* layer_norm_forward(PyObject*, PyObject* const* args, Py_ssize_t count, PyObject* keywords) {
+    PyObject* v[7];
+    if (!parse("layer_norm_forward", kNormNames, 1, args, count, keywords, v)) return nullptr;
+    return guarded([&] {
+        const Tensor x = tensor_of("x", v[0], false), w = tensor_of("weight", v[1], true), b = tensor_of("bias", v[2], true);
+        const double eps = number(v[3], 1e-5);
+        const Drop drop = drop_of(v[4], v[5], v[6]);
+        std::tuple<Tensor, Tensor, Tensor> out;
+        {
+            py::gil_scoped_release free;
+            at::AutoGradMode off(false);
+            check_x("x", x);
+            const auto [y, stats] = run_forward(x, w, b, eps, drop, true);
+            out = {y, stats.select(0, 0), stats.select(0, 1)};
+        }
+        return triple(out);
+    });
+}
+
+PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t count, PyObject* keywords) {
+    static const char* const names[] = {"dy", "x", "weight", "mean", "rstd", "dropout", "seed", "offset"};
+    PyObject* v[8];
+    if (!parse("layer_norm_backward", names, 5, args, count, keywords, v)) return nullptr;
+    return guarded([&] {
+        const Tensor dy = tensor_of("dy", v[0], false), x = tensor_of("x", v[1], false), w = tensor_of("weight", v[2], true);
+        const Tensor mean = tensor_of("mean", v[3], false), rstd = tensor_of("rstd", v[4], false);
+        const Drop drop = drop_of(v[5], v[6], v[7]);
+        std::tuple<Tensor, Tensor, Tensor> out;
+        {
+            py::gil_scoped_release free;
+            at::AutoGradMode off(false);
+            check_x("x", x);
+            check_x("dy", dy);
+            check_like("dy", dy, x);
+            if (dy.sizes() != x.sizes()) refuse("dy has the shape " + str(dy.sizes()) + ", x " + str(x.sizes()));
+            const auto wide = x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat;
+            const int64_t rows = x.numel() / x.size(-1);
+            for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"mean", mean}, {"rstd", rstd}})
+                if (t.device() != x.device() || t.scalar_type() != wide || !t.is_contiguous() || t.numel() != rows)
+                    refuse(std::string(name) + " is not the forward pass's: " + str(rows) + " numbers of " + str(wide) + " on " + str(x.device()));
+            out = run_backward(dy, x, w, mean.data_ptr(), rstd.data_ptr(), drop, true, true, true);
+        }
+        return triple(out);
+    });
 }
 
 template <class F>
@@ -349,17 +448,40 @@ void take(F& slot, const py::dict& addresses, const char* name) {
     slot = reinterpret_cast<F>(addresses[name].cast<uintptr_t>());
 }
 
+PyMethodDef functions[] = {
+    {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&dropout)), METH_FASTCALL | METH_KEYWORDS,
+     R"(dropout($module, x, p, seed, offset=0)
+--
+
+Each element dropped with probability p (rounded to a multiple of 2^-16), the others multiplied so that the mean
+stays; differentiable.  The mask is a function of (seed, offset, row, column) alone: calls that are to draw
+independently -- layers, steps -- take different offsets or seeds.  `offset` may be a tensor of one int64 on x's
+device, read when the kernels run: a captured graph then drops other elements on every replay if the program
+changes it between replays (not between a forward pass and its backward pass).)"},
+    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&layer_norm)), METH_FASTCALL | METH_KEYWORDS,
+     R"(layer_norm($module, x, weight=None, bias=None, eps=1e-05, dropout=0.0, seed=0, offset=0)
+--
+
+(h - mean h) / sqrt(mean (h - mean h)^2 + eps) * weight + bias over the last dimension, with h = x, or
+h = dropout(x, dropout, seed, offset) in the same pass; differentiable in x, weight and bias.  weight and bias hold
+x's type; sums are taken in float32 (float64 for float64) and y is rounded once.  Captured into a graph with its
+backward pass while an eager graph of the same leaves is alive, the call is refused.)"},
+    {"layer_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&layer_norm_forward)), METH_FASTCALL | METH_KEYWORDS,
+     R"(layer_norm_forward($module, x, weight=None, bias=None, eps=1e-05, dropout=0.0, seed=0, offset=0)
+--
+
+layer_norm without autograd: (y, mean, 1 / standard deviation), the latter two one number a row.)"},
+    {"layer_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&layer_norm_backward)), METH_FASTCALL | METH_KEYWORDS,
+     R"(layer_norm_backward($module, dy, x, weight, mean, rstd, dropout=0.0, seed=0, offset=0)
+--
+
+(dx, dweight, dbias) from dy and what layer_norm_forward took and gave; without autograd, so it can be captured
+into a graph whatever else holds on to the leaves.)"},
+    {nullptr, nullptr, 0, nullptr}};
+
 }  // namespace
 
 PYBIND11_MODULE(_layers, m) {
-    py::register_exception_translator([](std::exception_ptr e) {
-        try {
-            if (e) std::rethrow_exception(e);
-        } catch (const Failure& f) {
-            const py::object type = py::module_::import("epidemicsimulator_amd._capi").attr("EpiError");
-            PyErr_SetObject(type.ptr(), type(f.status, f.what()).ptr());
-        }
-    });
     m.def("bind", [](const py::dict& a) {
         take(lib.dropout, a, "epi_dropout");
         take(lib.forward, a, "epi_layer_norm_forward");
@@ -367,8 +489,5 @@ PYBIND11_MODULE(_layers, m) {
         take(lib.backward, a, "epi_layer_norm_backward");
         take(lib.last_error, a, "epi_last_error");
     });
-    m.def("dropout", &dropout);
-    m.def("layer_norm", &layer_norm);
-    m.def("layer_norm_forward", &layer_norm_forward);
-    m.def("layer_norm_backward", &layer_norm_backward);
+    if (PyModule_AddFunctions(m.ptr(), functions) != 0) throw py::error_already_set();
 }
