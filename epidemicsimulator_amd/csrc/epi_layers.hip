@@ -591,7 +591,7 @@ __global__ __launch_bounds__(256) void norm_forward_walk_kernel(NormArgs a) {
 // dx, TPR threads a row, in two walks (the two means; the result).  The others take columns, 32 of them and
 // seg_rows rows each, and form sums of dy u and dy: 4 threads side by side, 64 rows at a time, then the 64 sums of
 // every column in a fixed order.  With one segment they are the gradients, else partial sums for
-// norm_reduce_kernel.  For what the kernel below does not take: up to 1,024 rows, where one launch is what counts
+// norm_reduce_kernel.  For what the kernel below does not take: few rows (split_rows), where one launch is what counts
 // (512 x 128 double: 8 us, bound by a few loads one after the other), rows below eight columns, and rows beyond the
 // registers, whose x and dy are read twice from memory (1,000 x 100,000 bfloat16: 279 us, 2.2 TB/s over x, dy and dx).
 constexpr int kTileCols = 32, kTileSlots = 64;
@@ -1005,8 +1005,11 @@ int64_t backward_blocks(int64_t rows) {
                                       : (int64_t)1024 * 256 / norm_threads(TPR);
     return std::min((rows + kRows - 1) / kRows, most);
 }
-// Up to so many rows the split kernel does it all in one launch (1,536 x 128 float: 9.6 us there, 7.1 here).
-constexpr int64_t kSplitRows = 1024;
+// Up to so many rows the split kernel does it all in one launch: narrow rows until its column workgroups have walked
+// longer than a second launch takes (bfloat16 x 128: 768 rows 6.9 us split and 6.8 in two, 1,200 rows 10.1 and 7.0; x
+// 1,024: 1,024 rows 8.4 and 9.8), wide ones until reading x and dy twice does (x 4,096: 1,200 rows 17.7 and 26.7, 3,000
+// 35 and 32; x 8,192: 1,024 rows 24 and 30, 1,200 32 and 30).
+int64_t split_rows(int64_t cols) { return cols <= 512 ? 768 : cols > 1024 && cols <= 4096 ? 1536 : 1024; }
 
 // Threads of a row in the kernels for several networks at once, whose rows have up to 256 columns: one chunk each.
 template <class F>
@@ -1015,8 +1018,9 @@ void with_set_shape(int64_t cols, F f) {
     else f(int_c<32>{});
 }
 
-// Rows of one column workgroup: as many as keep its walk short; more rows than that become segments.
-constexpr int64_t kSegRows = 1024;
+// Rows of one column workgroup.  Up to 1,024 rows it takes them all and leaves the gradients themselves; beyond, where a
+// second launch sums segments anyway, they are short (1,200 x 2,048 bfloat16: 10.0 us, 13.0 with segments of 1,024).
+int64_t seg_rows(int64_t rows) { return rows <= 1024 ? 1024 : 512; }
 
 SplitShape split_shape(const NormArgs& a, int tpr) {
     SplitShape sh{};
@@ -1025,7 +1029,8 @@ SplitShape split_shape(const NormArgs& a, int tpr) {
     if (a.sets.count) {
         sh.segs = a.sets.count; sh.seg_rows = a.sets.set_rows;
     } else {
-        sh.segs = (a.rows + kSegRows - 1) / kSegRows; sh.seg_rows = kSegRows;
+        sh.seg_rows = seg_rows(a.rows);
+        sh.segs = (a.rows + sh.seg_rows - 1) / sh.seg_rows;
     }
     return sh;
 }
@@ -1103,12 +1108,12 @@ size_t norm_backward_workspace(LayerType type, int64_t rows, int64_t cols, bool 
     return with_type(type, [&](auto t) -> size_t {
         using T = decltype(t);
         int64_t parts = 0;
-        if (rows > kSplitRows)
+        if (rows > split_rows(cols))
             with_flag(drop, [&](auto on) {
                 with_row_shape<T, false, decltype(on)::value>(cols, [&](auto tpr, auto) { parts = backward_blocks<decltype(tpr)::value>(rows); });
             });
         if (!parts) {
-            const int64_t segs = (rows + kSegRows - 1) / kSegRows;
+            const int64_t segs = (rows + seg_rows(rows) - 1) / seg_rows(rows);
             parts = segs > 1 ? segs : 0;
         }
         return (size_t)parts * 2 * cols * sizeof(wide_t<T>);
@@ -1140,7 +1145,7 @@ hipError_t launch_norm_backward(LayerType type, const NormArgs& args, hipStream_
         int64_t parts = 0;
         with_flag(a.drop.threshold != 0, [&](auto drop) {
             constexpr bool D = decltype(drop)::value;
-            if (a.rows > kSplitRows)
+            if (a.rows > split_rows(a.cols))
                 with_row_shape<T, false, D>(a.cols, [&](auto tpr, auto nv) {
                     constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
                     NormArgs b = a;
@@ -1149,7 +1154,8 @@ hipError_t launch_norm_backward(LayerType type, const NormArgs& args, hipStream_
                     hipLaunchKernelGGL((norm_backward_kernel<T, TPR, NV, D>), dim3((unsigned)parts), dim3(norm_threads(TPR)), 0, s, b);
                 });
             if (parts) return;
-            // a thread for rows of one chunk, a workgroup for those of more than four chunks a lane
+            // a thread for rows of one chunk; a workgroup for those of more than four chunks a lane, and for those of
+            // more than one where rows are few (bfloat16, 64 x 2,048: 3.7 us, 6.4 with a wave a row; 1,024 x 2,048: 10.0, 8.7)
             const auto split = [&](auto tpr) {
                 constexpr int TPR = decltype(tpr)::value;
                 const SplitShape sh = split_shape(a, TPR);
@@ -1158,7 +1164,7 @@ hipError_t launch_norm_backward(LayerType type, const NormArgs& args, hipStream_
                 if (sh.segs > 1) parts = sh.segs;
             };
             if (a.cols <= kChunk) split(int_c<1>{});
-            else if (a.cols <= 2048) split(int_c<64>{});
+            else if (a.cols <= 512 || (a.cols <= 2048 && a.rows > 512)) split(int_c<64>{});
             else split(int_c<256>{});
         });
         if (parts && vectors)

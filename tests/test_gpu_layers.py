@@ -129,6 +129,7 @@ def test_norm_many_wide_rows(L, rows, cols, dtype):
 
 @pytest.mark.parametrize("dtype", list(TYPES.values()), ids=list(TYPES))
 @pytest.mark.parametrize("rows, cols", [(1100, 1536), (1100, 1537), (1050, 8193), (1050, 12001), (1030, 16384), (1030, 16392), (1026, 20003),
+                                        (768, 512), (769, 512), (769, 513), (1024, 1030), (1025, 4096), (1536, 2048), (1537, 2048), (512, 700), (513, 700),
                                         (1026, 24576), (1026, 24585), (1026, 7), (1026, 8), (1300, 1), (70000, 3)])
 def test_norm_backward_shapes_with_and_without_dropout(L, rows, cols, dtype):
     both_ways(L, dtype, rows, cols, 0.0)
