@@ -18,6 +18,7 @@
 #include <cmath>
 #include <cstring>
 #include <memory>
+#include <new>
 #include <thread>
 #include <vector>
 
@@ -1132,7 +1133,7 @@ EPI_API int32_t epi_agents_set_weights(epi_agents* g, int32_t agent, int32_t tar
     return EPI_OK;
 }
 
-EPI_API int32_t epi_agents_regularise(epi_agents* g, double dropout, double eps, int64_t seed) {
+EPI_API int32_t epi_agents_regularise(epi_agents* g, double dropout, double eps, int64_t seed) try {
     if (!g) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: null handle");
     if (!(dropout >= 0.0 && dropout < 1.0)) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: dropout %g outside [0,1)", dropout);
     if (!(eps > 0.0) || !std::isfinite(eps)) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: eps %g is not a positive number", eps);
@@ -1153,6 +1154,8 @@ EPI_API int32_t epi_agents_regularise(epi_agents* g, double dropout, double eps,
     g->norm_dropout = dropout; g->norm_eps = eps; g->norm_seed = seed;
     g->normed = true;
     return EPI_OK;
+} catch (const std::bad_alloc&) {
+    return fail(EPI_ERR_DEVICE, "agents_regularise: out of host memory");
 }
 
 EPI_API int32_t epi_agents_get_norm(epi_agents* g, int32_t agent, int32_t target, double* gain1, double* bias1, double* gain2, double* bias2) {
