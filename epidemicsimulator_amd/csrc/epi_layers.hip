@@ -348,7 +348,7 @@ struct DropShape {
 };
 
 template <class T, bool DROP>
-__global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, DropShape s, DropArgs d) {
+__global__ __launch_bounds__(256) void dropout_kernel(const T* x, T* y, DropShape s, DropArgs d) {
     const uint32_t g = blockIdx.x * 256u + threadIdx.x;
     if (g >= s.chunks) return;
     const uint32_t r = (uint32_t)(((uint64_t)g * s.magic) >> s.shift), c = g - r * s.per_row;
