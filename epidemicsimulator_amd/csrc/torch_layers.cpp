@@ -13,6 +13,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <optional>
 #include <string>
 #include <tuple>
 
@@ -71,25 +73,30 @@ void check_like(const char* name, const Tensor& t, const Tensor& x) {
     if (t.scalar_type() != x.scalar_type()) refuse(std::string(name) + " holds " + str(t.scalar_type()) + ", x holds " + str(x.scalar_type()));
 }
 
-// A tensor whose rows (the last dimension) are evenly spaced, and their distance: t itself, or a copy.
-std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
-    const int64_t cols = t.size(-1);
-    if (t.is_neg()) return {t.resolve_neg().contiguous(), cols};   // a view whose values are the memory's, negated
-    if (t.is_contiguous()) return {t, cols};
-    if (cols == 1 || t.stride(-1) == 1) {
-        // distance of the last leading dimension of more than one index; the others have to follow from it
-        int64_t step = cols, span = 0;
-        bool even = true;
-        for (int64_t d = t.dim() - 2; d >= 0 && even; --d) {
-            if (t.size(d) == 1) continue;
-            if (span == 0) { step = t.stride(d); span = step * t.size(d); }
-            else { even = t.stride(d) == span; span *= t.size(d); }
-        }
-        // rows of distance zero have a span of zero: only their neighbours' zero would follow
-        if (even && step > 0) return {t, step};
-        if (even && t.dim() == 2) return {t, step};
+// The distance between rows (the last dimension) that are evenly spaced over all leading dimensions, the last of them
+// running fastest; nothing where they are not, or where a row's columns do not lie next to each other.
+std::optional<int64_t> row_distance(at::IntArrayRef sizes, at::IntArrayRef strides) {
+    const int64_t cols = sizes.back();
+    if (std::find(sizes.begin(), sizes.end(), 0) != sizes.end()) return cols;   // no rows
+    if (cols != 1 && strides.back() != 1) return std::nullopt;
+    // The innermost leading dimension of more than one index sets the distance; the others have to follow from it.  A
+    // distance of zero counts like any other: what is expanded inside and moves outside is not evenly spaced.
+    int64_t step = cols, next = 0;
+    bool seen = false;
+    for (int64_t d = (int64_t)sizes.size() - 2; d >= 0; --d) {
+        if (sizes[d] == 1) continue;
+        if (!seen) { step = next = strides[d]; seen = true; }
+        if (strides[d] != next) return std::nullopt;
+        next *= sizes[d];
     }
-    return {t.contiguous(), cols};
+    return step;
+}
+
+// A tensor whose rows are evenly spaced, and their distance: t itself, or a copy.
+std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
+    if (t.is_neg()) return {t.resolve_neg().contiguous(), t.size(-1)};   // a view whose values are the memory's, negated
+    if (const auto step = row_distance(t.sizes(), t.strides())) return {t, *step};
+    return {t.contiguous(), t.size(-1)};
 }
 
 Tensor vector_of(const char* name, const Tensor& w, const Tensor& x) {
@@ -489,5 +496,7 @@ PYBIND11_MODULE(_layers, m) {
         take(lib.backward, a, "epi_layer_norm_backward");
         take(lib.last_error, a, "epi_last_error");
     });
+    // which tensors the calls read where they are, for tests without a GPU
+    m.def("row_distance", [](const Tensor& t) { return row_distance(t.sizes(), t.strides()); });
     if (PyModule_AddFunctions(m.ptr(), functions) != 0) throw py::error_already_set();
 }

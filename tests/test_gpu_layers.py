@@ -285,6 +285,51 @@ def test_strided_expanded_and_transposed_rows(L):
         assert torch.equal(L.dropout(x, 0.25, 4), L.dropout(x.contiguous(), 0.25, 4))
 
 
+def plain_copy(t):
+    """The same values, contiguous."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_gradients_expanded_in_a_middle_dimension(L, dtype):
+    """Sums over a leading dimension hand the backward pass a dy whose strides are zero there, inside or outside of others."""
+    x, w, b, dy = make(24, 128, dtype, 34)
+    f = R.factors(24, 128, 0.25, 4, 0)
+    for over in (0, 1, 2, (0, 1), (1, 2), (0, 2), (0, 1, 2)):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+        y = L.layer_norm(leaves[0].view(2, 3, 4, 128), leaves[1], leaves[2], dropout=0.25, seed=4)
+        weights = dy[:y.sum(over).numel() // 128].view(y.sum(over).shape)
+        got = torch.autograd.grad((y.sum(over) * weights).sum(), leaves)
+        full = plain_copy(weights.reshape([1 if d == over or (isinstance(over, tuple) and d in over) else n for d, n in enumerate((2, 3, 4, 128))])
+                          .expand(2, 3, 4, 128)).view(24, 128)
+        check_norm(dtype, x, w, b, full, 1e-5, f, y.view(24, 128), *got)
+        z = L.dropout(leaves[0].view(2, 3, 4, 128), 0.25, 4)
+        g, = torch.autograd.grad((z.sum(over) * weights).sum(), leaves[:1])
+        assert torch.equal(g, L.dropout(full, 0.25, 4))
+
+
+def test_inputs_expanded_in_a_middle_dimension(L):
+    x, w, b, dy = make(24, 96, torch.float32, 35)
+    views = [x[:5, None].expand(5, 7, 96), x[:5, None, None].expand(5, 2, 3, 96), x[:6].view(2, 3, 1, 96).expand(2, 3, 4, 96),
+             x[:6].view(2, 1, 3, 96).expand(2, 5, 3, 96), x[:4][None].expand(3, 4, 96), x[:1, None].expand(3, 4, 96), x[:4, :1, None].expand(4, 3, 96),
+             x[:3, None, :1].expand(3, 4, 1)]
+    for v in views:
+        rows, cols = v.numel() // v.shape[-1], v.shape[-1]
+        c = plain_copy(v)
+        d = torch.randn(v.shape, device="cuda")
+        e = dy[:v.shape[0], None, :cols].expand(v.shape) if v.dim() == 3 else d[:, :1].expand(v.shape)
+        assert torch.equal(L.dropout(v, 0.25, 4), L.dropout(c, 0.25, 4))
+        ww, bb = w[:cols].contiguous(), b[:cols].contiguous()
+        got, want = L.layer_norm_forward(v, ww, bb, dropout=0.25, seed=4), L.layer_norm_forward(c, ww, bb, dropout=0.25, seed=4)
+        for p, q in zip(got, want):
+            assert torch.equal(p, q)
+        for g in (d, e):
+            for p, q in zip(L.layer_norm_backward(g, v, ww, *want[1:], dropout=0.25, seed=4),
+                            L.layer_norm_backward(plain_copy(g), c, ww, *want[1:], dropout=0.25, seed=4)):
+                assert torch.equal(p, q)
+        check_norm(torch.float32, c.view(rows, cols), ww, bb, None, 1e-5, R.factors(rows, cols, 0.25, 4, 0), got[0].view(rows, cols))
+
+
 def test_more_dimensions_and_one(L):
     x, w, b, dy = make(24, 50, torch.float32, 32)
     y = L.layer_norm(x, w, b)

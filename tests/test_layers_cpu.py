@@ -187,3 +187,50 @@ def test_public_names_are_documented():
     from epidemicsimulator_amd import layers
     for name in layers.__all__:
         assert inspect.getdoc(getattr(layers, name))
+
+
+def layouts():
+    """Tensors of two to four dimensions over small storages: permuted, sliced, expanded, single columns and rows, none."""
+    import itertools
+    for sizes in ((5, 8), (6, 1), (1, 8), (4, 3, 8), (2, 3, 1), (1, 5, 7), (3, 1, 9), (0, 3, 8), (3, 0, 8), (2, 3, 4, 5), (2, 1, 3, 8), (1, 3, 1, 2), (2, 2, 2, 1)):
+        t = torch.arange(float(np.prod(sizes))).view(sizes)
+        views = [t.permute(order) for order in itertools.permutations(range(t.dim()))]
+        views += [t[tuple(slice(None, None, step) for step in steps)] for steps in itertools.product((1, 2), repeat=t.dim())]
+        views += [t.narrow(d, 1, t.shape[d] - 1) for d in range(t.dim()) if t.shape[d] > 1]
+        for v in views:
+            yield v
+            for ones in itertools.product((False, True), repeat=v.dim()):   # one index of some dimensions, expanded again
+                if v.numel():
+                    w = v[tuple(slice(0, 1) if one else slice(None) for one in ones)]
+                    yield w
+                    yield w.expand([4 if n == 1 else n for n in w.shape])
+                    yield w.expand([3 if one else n for one, n in zip(ones, w.shape)])
+            for d in range(v.dim() + 1):
+                u = v.unsqueeze(d)
+                yield u.expand([3 if k == d else n for k, n in enumerate(u.shape)])
+
+
+def test_rows_are_read_where_they_lie():
+    """The distance the binding answers, taken over the tensor's storage, gives the tensor's rows (as_strided refuses what
+    lies outside the storage); no answer means a copy, which contiguous tensors never need."""
+    from epidemicsimulator_amd import layers
+    answers = set()
+    for t in layouts():
+        step = layers._layers.row_distance(t)
+        answers.add((t.dim(), step is None, step == 0))
+        if step is None:
+            assert not t.is_contiguous()
+            continue
+        rows = t.numel() // t.shape[-1] if t.shape[-1] else 0
+        got = t.as_strided((rows, t.shape[-1]), (step, 1))
+        assert torch.equal(got, t.contiguous().view(rows, t.shape[-1])), (t.shape, t.stride(), step)
+    for dims in (2, 3, 4):
+        assert (dims, True, False) in answers and (dims, False, True) in answers and (dims, False, False) in answers
+
+
+@pytest.mark.parametrize("sizes, strides, want", [
+    ((4, 3, 128), (128, 0, 1), None), ((4, 3, 2, 128), (128, 0, 0, 1), None), ((4, 3, 128), (0, 128, 1), None), ((4, 3, 128), (0, 0, 1), 0),
+    ((4, 3, 128), (0, 0, 0), None), ((4, 3, 1), (1, 0, 0), None), ((4, 3, 128), (600, 200, 1), 200), ((4, 1, 128), (128, 0, 1), 128), ((4, 0, 8), (3, 7, 1), 8)])
+def test_expanded_dimensions_in_the_middle_are_copied(sizes, strides, want):
+    from epidemicsimulator_amd import layers
+    assert layers._layers.row_distance(torch.zeros(4000).as_strided(sizes, strides)) == want
