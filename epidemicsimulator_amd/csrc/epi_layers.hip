@@ -575,7 +575,7 @@ __device__ inline void norm_forward_row(const NormArgs& a, int64_t row, wide_t<T
     }
 }
 
-// A launch holds at most kMaxBlocks workgroups (a grid has fewer than 2^32 threads): they walk on over the rows.
+// A launch holds at most kMaxBlocks workgroups (a grid has fewer than 2^32 threads): they walk on over the rows or columns.
 constexpr int64_t kMaxBlocks = (int64_t)1 << 20;
 
 template <class T, int TPR, bool DROP, bool SETS>
@@ -908,21 +908,23 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const wide_t<T>* __re
     using A = wide_t<T>;
     __shared__ A lds[64][17];
     const int lane = threadIdx.x % 16, slot = threadIdx.x / 16;
-    const int64_t at = (int64_t)blockIdx.x * 16 + lane;   // over [2][cols]
-    A s = 0;
-    if (at < 2 * cols) {
+    for (int64_t tile = blockIdx.x; tile * 16 < 2 * cols; tile += gridDim.x) {
+        const int64_t at = tile * 16 + lane;   // over [2][cols]
+        A s = 0;
+        if (at < 2 * cols) {
 #pragma unroll 8
-        for (int64_t p = slot; p < parts; p += 64) s += part[p * 2 * cols + at];
-    }
-    lds[slot][lane] = s;
-    __syncthreads();
-    for (int half = 32; half > 0; half >>= 1) {
-        if (slot < half) lds[slot][lane] += lds[slot + half][lane];
+            for (int64_t p = slot; p < parts; p += 64) s += part[p * 2 * cols + at];
+        }
+        lds[slot][lane] = s;   // what others read of the tile before lies behind a barrier
         __syncthreads();
-    }
-    if (slot == 0 && at < 2 * cols) {
-        T* out = at < cols ? dweight : dbias;
-        if (out) out[at < cols ? at : at - cols] = (T)lds[0][lane];
+        for (int half = 32; half > 0; half >>= 1) {
+            if (slot < half) lds[slot][lane] += lds[slot + half][lane];
+            __syncthreads();
+        }
+        if (slot == 0 && at < 2 * cols) {
+            T* out = at < cols ? dweight : dbias;
+            if (out) out[at < cols ? at : at - cols] = (T)lds[0][lane];
+        }
     }
 }
 
@@ -1169,7 +1171,7 @@ hipError_t launch_norm_backward(LayerType type, const NormArgs& args, hipStream_
             else split(int_c<256>{});
         });
         if (parts && vectors)
-            hipLaunchKernelGGL(norm_reduce_kernel<T>, dim3((unsigned)((2 * a.cols + 15) / 16)), dim3(1024), 0, s,
+            hipLaunchKernelGGL(norm_reduce_kernel<T>, dim3((unsigned)std::min((2 * a.cols + 15) / 16, kMaxBlocks)), dim3(1024), 0, s,
                                static_cast<const wide_t<T>*>(a.workspace), parts, a.cols, static_cast<T*>(a.dweight),
                                static_cast<T*>(a.dbias));
     });

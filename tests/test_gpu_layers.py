@@ -442,6 +442,32 @@ def test_more_chunks_than_one_launch_holds(L):
         assert np.array_equal(host(y[start:start + 6]), R.apply_factors(host(x[:6]), f))
 
 
+def test_gradients_of_more_columns_than_a_grid_has_threads(L):
+    """dweight and dbias of 2^25 columns and more, in three segments of rows: the reduction walks over the columns.  Every
+    row is the same, with a mean and deviation of its own, so dweight = dy (x sum r - sum m r) and dbias = rows dy."""
+    import ctypes as C
+    from epidemicsimulator_amd import _capi
+    rows, cols = 1025, (1 << 25) + 19
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, dy = (torch.randn(cols, generator=g, device="cuda") for _ in range(2))
+    m = 0.5 * torch.randn(rows, generator=g, device="cuda")
+    r = 0.5 + torch.rand(rows, generator=g, device="cuda")
+    d = _capi.LayerDesc(rows=rows, cols=cols, eps=1e-5, dtype=1, device=0)
+    lib, need = _capi.lib(), C.c_size_t()
+    assert lib.epi_layer_norm_backward_workspace(C.byref(d), C.byref(need)) == 0
+    work = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    dw, db = torch.full_like(x, 7.0), torch.full_like(x, 7.0)
+    assert lib.epi_layer_norm_backward(C.byref(d), x.data_ptr(), dy.data_ptr(), None, m.data_ptr(), r.data_ptr(), None, dw.data_ptr(), db.data_ptr(),
+                                       work.data_ptr(), need.value, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    e, chain = inner(torch.float32), rows / 16 + 100
+    X, D, s, t = x.double(), dy.double(), r.double().sum(), (m.double() * r.double()).sum()
+    want = D * (X * s - t)
+    size = D.abs() * (X.abs() * s + (m.double() * r.double()).abs().sum())
+    assert bool(((dw.double() - want).abs() <= e * want.abs() + 4 * e * chain * size).all())
+    assert bool(((db.double() - rows * D).abs() <= e * (1 + chain) * rows * D.abs()).all())
+
+
 def test_negated_views(L):
     z = torch.conj(torch.complex(torch.randn(5, 20), torch.randn(5, 20)).cuda())
     x = z.imag
