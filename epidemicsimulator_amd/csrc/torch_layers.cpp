@@ -189,6 +189,14 @@ variable_list once(variable_list grads, bool again) {
     return (*error)(std::move(grads));
 }
 
+// Gradients are taken backwards only: the tangent of a dual tensor (forward-mode derivatives) would be lost, which reads
+// as a derivative of zero.  Refused, unless forward mode is switched off.
+template <class... T>
+void refuse_tangents(const T&... inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    if (((inputs.defined() && inputs._fw_grad(/*level=*/0).defined()) || ...)) refuse("layer operators have no forward-mode derivatives");
+}
+
 // The nodes of the graph, with what their backward passes need.
 struct DropoutNode : torch::autograd::Node {
     Drop drop;
@@ -198,6 +206,7 @@ struct DropoutNode : torch::autograd::Node {
         at::AutoGradMode off(false);
         variable_list out(1);
         if (grads[0].defined()) {
+            refuse_tangents(grads[0]);
             Drop d = drop;
             d.offset_dev = offset_dev.unpack();
             out[0] = run_dropout(grads[0], d);
@@ -217,6 +226,7 @@ struct NormNode : torch::autograd::Node {
         at::AutoGradMode off(false);
         variable_list out(3);
         if (grads[0].defined()) {
+            refuse_tangents(grads[0]);
             const Tensor s = stats.unpack();
             Drop d = drop;
             d.offset_dev = offset_dev.unpack();
@@ -377,6 +387,7 @@ PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t count, PyObject* 
         Tensor y;
         {
             py::gil_scoped_release free;
+            refuse_tangents(x);
             check_x("x", x);
             y = at::GradMode::is_enabled() && wants(x) ? record_dropout(x, drop) : run_dropout(x, drop);
         }
@@ -396,6 +407,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t count, PyObjec
         Tensor y;
         {
             py::gil_scoped_release free;
+            refuse_tangents(x, w, b);
             check_x("x", x);
             y = at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b)) ? record_norm(x, w, b, eps, drop)
                                                                                 : run_forward(x, w, b, eps, drop, false).first;
@@ -461,7 +473,7 @@ PyMethodDef functions[] = {
 --
 
 Each element dropped with probability p (rounded to a multiple of 2^-16), the others multiplied so that the mean
-stays; differentiable.  The mask is a function of (seed, offset, row, column) alone: calls that are to draw
+stays; differentiable, backwards.  The mask is a function of (seed, offset, row, column) alone: calls that are to draw
 independently -- layers, steps -- take different offsets or seeds.  `offset` may be a tensor of one int64 on x's
 device, read when the kernels run: a captured graph then drops other elements on every replay if the program
 changes it between replays (not between a forward pass and its backward pass).)"},
@@ -470,7 +482,7 @@ changes it between replays (not between a forward pass and its backward pass).)"
 --
 
 (h - mean h) / sqrt(mean (h - mean h)^2 + eps) * weight + bias over the last dimension, with h = x, or
-h = dropout(x, dropout, seed, offset) in the same pass; differentiable in x, weight and bias.  weight and bias hold
+h = dropout(x, dropout, seed, offset) in the same pass; differentiable, backwards, in x, weight and bias.  weight and bias hold
 x's type; sums are taken in float32 (float64 for float64) and y is rounded once.  Captured into a graph with its
 backward pass while an eager graph of the same leaves is alive, the call is refused.)"},
     {"layer_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&layer_norm_forward)), METH_FASTCALL | METH_KEYWORDS,

@@ -271,6 +271,24 @@ def test_the_graph_keeps_autograds_rules(L):
         assert torch.equal(L.layer_norm(x.clone(), w.clone(), b.clone()), L.layer_norm_forward(x, w, b)[0])
 
 
+def test_tangents_are_refused(L):
+    """Forward-mode derivatives, of the inputs and of the gradient that a backward pass is given."""
+    import torch.autograd.forward_ad as forward_ad
+    from epidemicsimulator_amd import _capi
+    x, w, b, dy = make(6, 40, torch.float32, 23)
+    x.requires_grad_(True)
+    with forward_ad.dual_level():
+        for t in ([forward_ad.make_dual(x, dy), w, b], [x, forward_ad.make_dual(w, w), b], [x, w, forward_ad.make_dual(b, b)]):
+            with pytest.raises(_capi.EpiError, match="forward-mode"):
+                L.layer_norm(*t)
+        with pytest.raises(_capi.EpiError, match="forward-mode"):
+            L.dropout(forward_ad.make_dual(x, dy), 0.5, 1)
+        for y in (L.layer_norm(x, w, b), L.dropout(x, 0.5, 1)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, x, forward_ad.make_dual(dy, dy), retain_graph=True)
+            torch.autograd.grad(y, x, dy)
+
+
 # ---- layouts -------------------------------------------------------------------------------------------
 def test_strided_expanded_and_transposed_rows(L):
     wide, w, b, dyw = make(40, 300, torch.float32, 31)

@@ -172,6 +172,22 @@ def test_python_refuses_tensors_that_are_not_on_a_gpu():
         assert e.value.status == BAD
 
 
+def test_tangents_are_refused():
+    """The tangent of a dual tensor would be lost and read as zero; seen before anything else, so without a GPU too."""
+    import torch.autograd.forward_ad as forward_ad
+    from epidemicsimulator_amd import layers
+    x, w = torch.ones(3, 8), torch.ones(8)
+    with forward_ad.dual_level():
+        t, v = forward_ad.make_dual(x, torch.ones(3, 8)), forward_ad.make_dual(w, torch.ones(8))
+        for f in (lambda: layers.dropout(t, 0.1, 1), lambda: layers.layer_norm(t), lambda: layers.layer_norm(x, v), lambda: layers.layer_norm(x, None, v)):
+            with pytest.raises(_capi.EpiError, match="forward-mode"):
+                f()
+            with torch.no_grad(), pytest.raises(_capi.EpiError, match="forward-mode"):
+                f()
+            with forward_ad._set_fwd_grad_enabled(False), pytest.raises(_capi.EpiError, match="on the GPU only"):
+                f()
+
+
 def test_two_hip_runtimes_are_refused():
     """libepi.so loaded before torch: the binding says so instead of mixing the two (in a process of its own)."""
     import subprocess
