@@ -14,6 +14,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <mutex>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -197,11 +198,13 @@ void refuse_tangents(const T&... inputs) {
     if (((inputs.defined() && inputs._fw_grad(/*level=*/0).defined()) || ...)) refuse("layer operators have no forward-mode derivatives");
 }
 
-// The nodes of the graph, with what their backward passes need.
+// The nodes of the graph, with what their backward passes need; a pass holds the node's mutex, so that one that releases
+// the graph's tensors waits for another that reads them.
 struct DropoutNode : torch::autograd::Node {
     Drop drop;
     SavedVariable offset_dev;
     variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
         const bool again = at::GradMode::is_enabled();
         at::AutoGradMode off(false);
         variable_list out(1);
@@ -214,7 +217,10 @@ struct DropoutNode : torch::autograd::Node {
         at::AutoGradMode on(again);
         return once(std::move(out), again);
     }
-    void release_variables() override { offset_dev.reset_data(); }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        offset_dev.reset_data();
+    }
     std::string name() const override { return "EpiDropoutBackward"; }
 };
 
@@ -222,6 +228,7 @@ struct NormNode : torch::autograd::Node {
     Drop drop;
     SavedVariable x, weight, stats, offset_dev;
     variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
         const bool again = at::GradMode::is_enabled();
         at::AutoGradMode off(false);
         variable_list out(3);
@@ -239,6 +246,7 @@ struct NormNode : torch::autograd::Node {
         return once(std::move(out), again);
     }
     void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
         x.reset_data(); weight.reset_data(); stats.reset_data(); offset_dev.reset_data();
     }
     std::string name() const override { return "EpiLayerNormBackward"; }

@@ -526,6 +526,34 @@ def test_two_streams_at_once(L):
                 assert torch.equal(p, q)
 
 
+def test_two_threads_backward_over_one_graph(L):
+    """Some calls keep the graph's tensors and one lets them go: each has the right gradients, or an error that says so."""
+    import threading
+    x, w, b, dy = make(300, 96, torch.float32, 73)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(L.layer_norm(x, w, b, dropout=0.1, seed=2), leaves, dy)
+    for _ in range(20):
+        y = L.layer_norm(x, w, b, dropout=0.1, seed=2)
+        wrong, right = [], []
+
+        def work(keep):
+            for k in range(5):
+                try:
+                    got = torch.autograd.grad(y, leaves, dy, retain_graph=keep or k < 4)
+                except RuntimeError as e:
+                    if "second time" not in str(e):
+                        wrong.append(e)
+                    return
+                (right if all(torch.equal(p, q) for p, q in zip(got, want)) else wrong).append(k)
+
+        threads = [threading.Thread(target=work, args=(k == 0,)) for k in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong and len(right) >= 5
+
+
 def test_captured_graphs_replayed_on_new_inputs(L):
     """Two graphs of the same calls with an eager call between the replays; the masks follow the offset's value."""
     def record(rows, cols):
