@@ -254,13 +254,15 @@ struct NormNode : torch::autograd::Node {
 
 // A leaf that an eager graph still holds collects its gradient on that graph's stream.  A backward pass captured into a
 // HIP graph meanwhile would wait across the two streams, which is no part of a capture and ends the process: refused
-// while the forward pass is being captured.
-void check_capture(std::initializer_list<Tensor> leaves, const Tensor& x) {
+// while the forward pass is being captured, for the leaves among the inputs and those that the inputs are views of.
+void check_capture(std::initializer_list<Tensor> inputs, const Tensor& x) {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     const auto here = c10::hip::getCurrentHIPStream(x.get_device()).id();
-    for (const Tensor& t : leaves) {
-        if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
-        const auto collects = torch::autograd::impl::try_get_grad_accumulator(t);
+    for (const Tensor& t : inputs) {
+        if (!t.defined() || !t.requires_grad()) continue;
+        const Tensor leaf = !t.is_leaf() && t.is_view() ? Tensor(t._base()) : t;
+        if (!leaf.is_leaf() || !leaf.requires_grad()) continue;
+        const auto collects = torch::autograd::impl::try_get_grad_accumulator(leaf);
         if (collects && collects->stream() && collects->stream()->id() != here)
             refuse("an eager graph of the same leaf is alive: drop its outputs before capturing, or capture layer_norm_forward and layer_norm_backward");
     }
@@ -492,7 +494,8 @@ changes it between replays (not between a forward pass and its backward pass).)"
 (h - mean h) / sqrt(mean (h - mean h)^2 + eps) * weight + bias over the last dimension, with h = x, or
 h = dropout(x, dropout, seed, offset) in the same pass; differentiable, backwards, in x, weight and bias.  weight and bias hold
 x's type; sums are taken in float32 (float64 for float64) and y is rounded once.  Captured into a graph with its
-backward pass while an eager graph of the same leaves is alive, the call is refused.)"},
+backward pass while an eager graph of the same leaves is alive, the call is refused: of the leaves that it is given or
+given views of; further up, other operators meet the same limit of captures.)"},
     {"layer_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&layer_norm_forward)), METH_FASTCALL | METH_KEYWORDS,
      R"(layer_norm_forward($module, x, weight=None, bias=None, eps=1e-05, dropout=0.0, seed=0, offset=0)
 --

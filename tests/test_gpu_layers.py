@@ -642,6 +642,30 @@ def test_capture_beside_an_eager_graph_of_the_leaves_is_refused(L):
     del alive
 
 
+def test_capture_beside_an_eager_graph_of_a_views_leaf_is_refused(L):
+    """Weights and inputs that are views of a leaf: the leaf behind them counts.  Nothing is differentiated in the capture."""
+    from epidemicsimulator_amd import _capi
+    x, _, _, _ = make(24, 128, torch.float32, 74)
+    flat = torch.randn(256, device="cuda", requires_grad=True)
+    leaf = x.clone().requires_grad_(True)
+    calls = [lambda: L.layer_norm(x, flat[:128], flat[128:]), lambda: L.layer_norm(x, None, flat.view(2, 128)[1]), lambda: L.layer_norm(leaf.view(2, 3, 4, 128)),
+             lambda: L.dropout(leaf[::2], 0.5, 1)]
+    alive = [f() for f in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for f in calls:
+            with pytest.raises(_capi.EpiError, match="eager graph"):
+                f()
+        with torch.no_grad():
+            out = [f() for f in calls]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, alive):
+            assert torch.equal(p, q)
+
+
 # ---- refusals ------------------------------------------------------------------------------------------------
 def test_refusals_of_tensors(L):
     from epidemicsimulator_amd import _capi
