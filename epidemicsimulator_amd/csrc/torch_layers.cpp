@@ -464,7 +464,7 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t count
             const auto wide = x.scalar_type() == at::kDouble ? at::kDouble : at::kFloat;
             const int64_t rows = x.numel() / x.size(-1);
             for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"mean", mean}, {"rstd", rstd}})
-                if (t.device() != x.device() || t.scalar_type() != wide || !t.is_contiguous() || t.numel() != rows)
+                if (t.device() != x.device() || t.scalar_type() != wide || !t.is_contiguous() || t.is_neg() || t.numel() != rows)
                     refuse(std::string(name) + " is not the forward pass's: " + str(rows) + " numbers of " + str(wide) + " on " + str(x.device()));
             out = run_backward(dy, x, w, mean.data_ptr(), rstd.data_ptr(), drop, true, true, true);
         }
