@@ -1224,7 +1224,10 @@ int32_t check_plane(const char* who, const char* name, const void* p, int64_t ro
     if (rows == 0) return EPI_OK;
     if (!p) return fail(EPI_ERR_BAD_ARGUMENT, "%s: %s is null", who, name);
     if (reinterpret_cast<uintptr_t>(p) % size) return fail(EPI_ERR_BAD_ARGUMENT, "%s: %s is not aligned to its elements", who, name);
-    if (rows > 1 && (stride < 0 || (written && stride < cols) || stride >= (int64_t)1 << 40))
+    int64_t last, bytes;   // the rows end within 2^63 bytes
+    if (rows > 1 && (stride < 0 || (written && stride < cols) || stride >= (int64_t)1 << 40 ||
+                     __builtin_mul_overflow(rows - 1, stride, &last) || __builtin_add_overflow(last, cols, &last) ||
+                     __builtin_mul_overflow(last, size, &bytes)))
         return fail(EPI_ERR_BAD_ARGUMENT, "%s: %s has a row stride of %lld for %lld columns", who, name, (long long)stride, (long long)cols);
     return EPI_OK;
 }

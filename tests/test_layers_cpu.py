@@ -102,6 +102,20 @@ def test_wrong_strides_are_refused(wrong):
     refused(BAD, "epi_layer_norm_forward", C.byref(desc(**wrong)), ADDR[0], N, N, ADDR[1], N, N, N)
 
 
+@pytest.mark.parametrize("name", ["x_stride", "y_stride"])
+def test_rows_beyond_the_address_space_are_refused(name):
+    """2^31 - 1 rows, 2^38 elements apart, end behind 2^63 bytes: their extent is not taken modulo 2^64.  2^31 - 1 rows
+    2^29 apart end below 2^63: the call goes on to the overlap of x and y."""
+    rows = (1 << 31) - 1
+    x, y = (1 << 20, 1 << 40) if name == "x_stride" else (1 << 40, 1 << 20)
+    for stride, why in ((1 << 38, "row stride"), ((1 << 40) - 1, "row stride"), (1 << 62, "row stride"), (1 << 29, "overlap")):
+        d = desc(rows=rows, **{name: stride})
+        refused(BAD, "epi_dropout", C.byref(d), x, y, N)
+        assert why in _capi.last_error()
+        refused(BAD, "epi_layer_norm_forward", C.byref(d), x, N, N, y, N, N, N)
+        assert why in _capi.last_error()
+
+
 def test_misaligned_arrays_are_refused():
     d = C.byref(desc())
     refused(BAD, "epi_dropout", d, ADDR[0] + 2, ADDR[1], N)
