@@ -1135,7 +1135,9 @@ EPI_API int32_t epi_agents_set_weights(epi_agents* g, int32_t agent, int32_t tar
 
 EPI_API int32_t epi_agents_regularise(epi_agents* g, double dropout, double eps, int64_t seed) try {
     if (!g) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: null handle");
-    if (!(dropout >= 0.0 && dropout < 1.0)) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: dropout %g outside [0,1)", dropout);
+    // rounded to 2^-16, as the generator takes it: 1 would leave nothing of the trained pass
+    if (!(dropout >= 0.0 && dropout < 1.0) || make_drop(dropout, 0, 0, nullptr).threshold > 65535)
+        return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: dropout %g outside [0,1), or 1 when rounded to a multiple of 2^-16", dropout);
     if (!(eps > 0.0) || !std::isfinite(eps)) return fail(EPI_ERR_BAD_ARGUMENT, "agents_regularise: eps %g is not a positive number", eps);
     if (int32_t rc = use_device(g->device)) return rc;
     HIP_TRY(hipStreamSynchronize(g->stream));

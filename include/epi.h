@@ -404,14 +404,15 @@ int32_t epi_agents_set_weights(epi_agents *g, int32_t agent, int32_t target, con
                                const double *W2, const double *b2, const double *W3, const double *b3);
 /* Optional (no counterpart in the reference): layer norms and dropout in both hidden layers of every network of the
  * handle, h = relu(norm(dropout(W x + b))), with gains (one at first) and biases (zero) that learn with the other
- * weights.  Dropout, with probability `dropout` in [0, 1), acts on the trained pass of epi_agents_learn alone: the
- * target's passes, epi_agents_q_values and the rollouts of epi_world_rollout_greedy have the norms only.  In these
- * networks the derivative of the ReLU is 1 or 0 (the reference's trainBatch multiplies by the activation's value,
- * MLP.scala:44-58, and plain networks do so too).  The masks are epi_dropout's for `seed`: sample r of an agent is row
- * r, and layer l of its c-th learn step since this call (both from 0) has the offset (agent << 32) + 2 c + l.  The
- * weights stay as they are; calling it again starts gains, biases and masks afresh.  `eps` > 0 as in
- * epi_layer_norm_forward.  epi_world_set_mlp and epi_mlp_greedy_batch know plain networks only: the weights of
- * epi_agents_get_weights without their norms are another network.  Results are those of the formulas in doubles, not of a fixed order of operations. */
+ * weights.  Dropout, with probability `dropout` in [0, 1), and below 1 when rounded to 2^-16, acts on the trained
+ * pass of epi_agents_learn alone: the target's passes, epi_agents_q_values and the rollouts of
+ * epi_world_rollout_greedy have the norms only.  In these networks the derivative of the ReLU is 1 or 0 (the
+ * reference's trainBatch multiplies by the activation's value, MLP.scala:44-58, and plain networks do so too).  The
+ * masks are epi_dropout's for `seed`: sample r of an agent is row r, and layer l of its c-th learn step since this
+ * call (both from 0) has the offset (agent << 32) + 2 c + l.  The weights stay as they are; calling it again starts
+ * gains, biases and masks afresh.  `eps` > 0 as in epi_layer_norm_forward.  epi_world_set_mlp and
+ * epi_mlp_greedy_batch know plain networks only: the weights of epi_agents_get_weights without their norms are
+ * another network.  Results are those of the formulas in doubles, not of a fixed order of operations. */
 int32_t epi_agents_regularise(epi_agents *g, double dropout, double eps, int64_t seed);
 /* Gains and biases of both norms, [h] each (any get pointer may be NULL). */
 int32_t epi_agents_get_norm(epi_agents *g, int32_t agent, int32_t target, double *gain1, double *bias1, double *gain2,

@@ -262,6 +262,31 @@ def test_refusals(epi):
         world.regularise(0.1)
 
 
+def test_a_dropout_that_rounds_to_one_is_refused(epi):
+    """The generator takes p in units of 2^-16: 1 - 2^-17 rounds to 1 (halves to even) and would drop every unit of the trained
+    pass.  The largest p below it learns."""
+    hp = epi.HyperParams(hidden=16, batch_size=4, replay_capacity=50)
+    pool = epi.Agents([hp], max_grad_accum=1)
+    for p in (1.0 - 2.0 ** -17, 1.0 - 2.0 ** -20, np.nextafter(1.0, 0.0)):
+        assert R.threshold(p) == 65536
+        with pytest.raises(epi.EpiError):
+            pool.regularise(p)
+    with pytest.raises(epi.EpiError):
+        pool.norms(0)   # a refused call leaves the networks plain
+    p = 1.0 - 2.0 ** -16
+    assert R.threshold(p) == 65535
+    pool.regularise(p, 1e-5, 4)
+    feed(epi, np.random.default_rng(2), (pool,), 1, 10)
+    loss, _ = pool.learn([1], [4], 1)
+    assert np.isfinite(loss[0])
+    gains = [1 + 0.1 * np.arange(16.0)] * 4
+    pool.set_norms(0, gains)
+    for bad in (1.0, 1.0 - 2.0 ** -17):
+        with pytest.raises(epi.EpiError):
+            pool.regularise(bad)
+        assert all(np.array_equal(g, w) for g, w in zip(pool.norms(0), gains))   # and regularised ones as they are
+
+
 def test_a_world_whose_agents_are_regularised(epi):
     """stepOne until the agents have learned several times, the greedy evaluation on the device, and the same evaluation
     step by step through the agents' Q-values."""
