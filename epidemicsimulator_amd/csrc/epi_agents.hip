@@ -20,6 +20,7 @@
 #include <memory>
 #include <new>
 #include <thread>
+#include <utility>
 #include <vector>
 
 #include "../../include/epi.h"
@@ -1145,14 +1146,15 @@ EPI_API int32_t epi_agents_regularise(epi_agents* g, double dropout, double eps,
     std::vector<double> params(n * 8 * Hp, 0.0);   // gains one, biases zero, nothing behind the last unit
     for (size_t k = 0; k < n * 4; ++k)
         for (size_t u = 0; u < H; ++u) params[k * 2 * Hp + u] = 1.0;
-    g->normed = false;   // until everything is there
     HIP_TRY(g->Z1.ensure(3 * plane)); HIP_TRY(g->Z2.ensure(3 * plane));
     HIP_TRY(g->Y1.ensure(3 * plane)); HIP_TRY(g->Y2.ensure(3 * plane));
     HIP_TRY(g->DY.ensure(plane)); HIP_TRY(g->norm_sums.ensure(4 * n * H * 8));
     HIP_TRY(g->norm_stats.ensure(4 * n * g->Bp * 8));
     HIP_TRY(g->set_index.ensure(3 * n * 4)); HIP_TRY(g->set_used.ensure(3 * n * 4)); HIP_TRY(g->set_ctr.ensure(4 * n * 4));
-    HIP_TRY(g->norm.upload(params));
+    DevBuf norm;   // takes the old one's place when everything is there: a call that fails leaves the networks as they were
+    HIP_TRY(norm.upload(params));
     g->learns.assign(n, 0);
+    std::swap(g->norm.p, norm.p); std::swap(g->norm.bytes, norm.bytes);
     g->norm_dropout = dropout; g->norm_eps = eps; g->norm_seed = seed;
     g->normed = true;
     return EPI_OK;

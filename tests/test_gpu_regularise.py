@@ -262,6 +262,34 @@ def test_refusals(epi):
         world.regularise(0.1)
 
 
+def test_regularised_again_starts_afresh(epi):
+    """Gains, biases and masks of a second call are those of a first one; the weights stay."""
+    hp = epi.HyperParams(hidden=32, batch_size=8, replay_capacity=100, lr=0.05)
+    pools = [epi.Agents([hp] * 2, max_grad_accum=1) for _ in range(2)]
+    feed(epi, np.random.default_rng(4), pools, 2, 20)
+    rng = np.random.default_rng(5)
+    W = [rng.normal(size=w.shape) for w in pools[0].weights(0)]
+    for p in pools:
+        p.regularise(0.2, 1e-5, 9)
+        p.learn([1, 1], [8, 8], 1)
+    pools[0].learn([2, 2], [8, 8], 1)
+    pools[1].learn([2, 2], [8, 8], 1, [1, 0])
+    pools[0].regularise(0.3, 1e-4, 6)
+    pools[0].regularise(0.2, 1e-5, 9)
+    pools[1].regularise(0.2, 1e-5, 9)
+    for p in pools:
+        for a in range(2):
+            for target in (False, True):
+                g1, b1, g2, b2 = p.norms(a, target)
+                assert np.all(g1 == 1) and np.all(g2 == 1) and not b1.any() and not b2.any()
+                p.set_weights(a, W, target)
+        p.learn([3, 3], [8, 8], 1)
+    for a in range(2):
+        for g, w in zip(pools[0].weights(a) + pools[0].norms(a), pools[1].weights(a) + pools[1].norms(a)):
+            assert np.array_equal(g, w)
+        assert any(not np.array_equal(g, w) for g, w in zip(pools[0].weights(a), W))
+
+
 def test_a_dropout_that_rounds_to_one_is_refused(epi):
     """The generator takes p in units of 2^-16: 1 - 2^-17 rounds to 1 (halves to even) and would drop every unit of the trained
     pass.  The largest p below it learns."""
