@@ -343,6 +343,50 @@ def test_a_world_whose_agents_are_regularised(epi):
         assert [nd.s.i for nd in again.nodes] == list(out["i_series"][k, 0]), "step %d" % k
 
 
+@pytest.mark.parametrize("hidden, batch", [(64, 130), (128, 9), (100, 33), (256, 2)])
+def test_rollouts_of_batched_worlds(epi, hidden, batch):
+    """Instances in different states, each asking its node's regularised network on the device, against the same steps with
+    the actions that the agents give each instance by itself."""
+    import ctypes as C
+    from epidemicsimulator_amd import synth
+    countries, xy = synth.make_countries(9, 78)
+    n, t_max, steps = len(countries), 60, 6
+    conn = synth.gravity_dense(countries, xy)
+    rng = np.random.default_rng(hidden + batch)
+    hp = epi.HyperParams(hidden=hidden)
+    pool = epi.Agents([hp] * n)
+    pool.regularise(0.2, 1e-4, 1)
+    for a in range(n):
+        pool.set_weights(a, [rng.normal(size=w.shape) * 0.3 for w in pool.weights(a)])
+        pool.set_norms(a, [1 + 0.3 * rng.normal(size=hidden), 0.3 * rng.normal(size=hidden), 1 + 0.3 * rng.normal(size=hidden), 0.3 * rng.normal(size=hidden)])
+
+    def world():
+        it = iter([epi.EpidemicEnv(0.25 + 0.01 * k, 0.12, 0.008, 0.04, 5.0, 0.0, c.name, 100 + k, profile=c) for k, c in enumerate(countries)])
+        w = epi.WorldToy(hp, epi.State(0, 0, 0, 0, 0, 10_000, 0, t_max, 42), 2, conn, make_env_for=lambda name, pop: next(it), validate=True,
+                         countries=countries, batch=batch, learning=False)
+        apart = np.random.default_rng(5)
+        for _ in range(4):
+            st, _ = w.step_arrays(apart.integers(0, 8, (batch, n)), apart.normal(size=(batch, n)), t_max)
+        return w, st
+
+    wa, _ = world()
+    series, last = np.zeros((steps, batch, n)), np.empty((batch, n), dtype=epi.WorldToy.STATE_DTYPE)
+    arr, pk = np.zeros((batch, n), dtype=np.int32), np.zeros((batch, n))
+    epi.check(epi.lib().epi_world_rollout_greedy(wa._h, pool._h, C.c_int32(steps), C.c_int32(t_max), series.ctypes.data, arr.ctypes.data,
+                                                 pk.ctypes.data, last.ctypes.data))
+    wb, st = world()
+    asked = set()
+    for k in range(steps):
+        acts = np.array([pool.q_values([epi.State(*(row[f] for f in ("s", "i", "r", "d", "v", "hosp_cap", "t", "t_max", "seed"))) for row in one])[1]
+                         for one in st])
+        asked |= set(acts.ravel().tolist())
+        st, _ = wb.step_arrays(acts, None, t_max)
+        np.testing.assert_array_equal(series[k], st["i"])
+    np.testing.assert_array_equal(last, st)
+    assert len(asked) > 2   # the networks do choose
+    wa.close(); wb.close()
+
+
 def test_a_network_of_the_operators_beside_batched_worlds(epi):
     """Features of 64 worlds of six countries through linear -> dropout -> norm -> ReLU twice to Q-values with the layer
     operators, a TD loss, its gradients against the formulas in doubles, and the greedy actions back into the worlds."""
