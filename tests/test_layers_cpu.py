@@ -264,3 +264,16 @@ def test_rows_are_read_where_they_lie():
 def test_expanded_dimensions_in_the_middle_are_copied(sizes, strides, want):
     from epidemicsimulator_amd import layers
     assert layers._layers.row_distance(torch.zeros(4000).as_strided(sizes, strides)) == want
+
+
+@pytest.mark.parametrize("installed", [True, False])
+def test_build_asks_for_the_binding_where_torch_is_installed(monkeypatch, installed):
+    """The library builds without torch, and then nothing loads the binding that was not built."""
+    import importlib.util
+    import __graft_entry__ as entry
+    commands, found = [], importlib.util.find_spec
+    monkeypatch.setattr(entry.subprocess, "check_call", lambda command, **kw: commands.append(" ".join(command)))
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: found(name, *a) if installed or name != "torch" else None)
+    entry.build()
+    assert any("csrc" in c for c in commands)
+    assert any("layers" in c for c in commands) == installed
