@@ -432,7 +432,9 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_kernel(NormArg
     constexpr int kRows = norm_threads(TPR) / TPR;
     constexpr bool kHold = NV == 1 && sizeof(T) < 8;   // registers for the weights
     // registers for the next row, where they are left: 1,024 threads have 128 each (1,021 x 20,000 float with dropout:
-    // 43.7 us with the next row's and spills, 38.4 without; without dropout 36.7 with and 36.6 without)
+    // 43.7 us with the next row's and spills, 38.4 without; without dropout 36.7 with and 36.6 without).  Rows of more than
+    // 24,576 doubles spill all the same, 152 bytes a lane, and with dropout 404, from 16,385 on 172: 1,500 x 30,000 take
+    // 256 us (2.8 TB/s) and 316, 2,000 x 20,000 179 (3.6) and 226
     constexpr bool kAhead = TPR < 1024 || (DROP ? NV < 4 && NV * sizeof(T) <= 8 : NV * sizeof(T) <= 16);
     __shared__ A lds[kRowLds<TPR, 2>];
     int flip = 0;
@@ -594,7 +596,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_forward_walk_kernel(No
 // every column in a fixed order.  With one segment they are the gradients, else partial sums for
 // norm_reduce_kernel.  For what the kernel below does not take: few rows (split_rows), where one launch is what counts
 // (512 x 128 double: 8 us, bound by a few loads one after the other), rows below eight columns, and rows beyond the
-// registers, whose x and dy are read twice from memory (1,000 x 100,000 bfloat16: 279 us, 2.2 TB/s over x, dy and dx).
+// registers, whose x and dy are read twice from memory (1,000 x 100,000 bfloat16: 292 us, 2.1 TB/s over x, dy and dx).
 constexpr int kTileCols = 32, kTileSlots = 64;
 
 struct SplitShape {
@@ -734,7 +736,10 @@ __global__ __launch_bounds__(256) void norm_backward_split_kernel(NormArgs a, Sp
 // reduction (5.1 TB/s over x, dy and dx), 16,384 x 4,096 bfloat16 91 us (4.4 TB/s: 5 of them are the reduction of 512
 // partial rows); beyond 8,192 columns by what a workgroup of 1,024 threads can hold (6,000 x 16,000 bfloat16: 158 us,
 // 3.6 TB/s; with dw's sums in registers 171; with dropout, where x and dy are fetched again for the second half, 176 --
-// held they take 207 for 16-bit types, but 155 against 164 for float at 4,000 x 12,000).
+// held they take 207 for 16-bit types, but 155 against 164 for float at 4,000 x 12,000).  Doubles with 1,024 threads
+// spill 48 bytes a lane (124 with dropout): 3,000 x 8,000 take 190 us with the reduction and 226, 115 at a copy's rate.
+// The mean is read as one number of the sums' type, without the remainder that the forward pass takes off as well: u is
+// off by up to half a step of |mean| times r, alike over a row.
 template <class T, int TPR, int NV, bool DROP>
 __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormArgs a) {
     using A = wide_t<T>;
@@ -901,7 +906,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void norm_backward_kernel(NormAr
 }
 
 // Sums the partial rows of the two gradients: 16 columns and 64 rows at a time, then the 64 sums in a fixed order.  A few
-// loads one after the other: 3 to 4 us for 512 rows of 128 or 256 columns, 7 for 4,096 columns (16 MB, in the caches).
+// loads one after the other: 2 to 4 us for 512 rows of 128 or 256 columns, 7 for 4,096 columns (16 MB, in the caches).
 template <class T>
 __global__ __launch_bounds__(1024) void norm_reduce_kernel(const wide_t<T>* __restrict__ part, int64_t parts, int64_t cols,
                                                            T* dweight, T* dbias) {
@@ -961,7 +966,7 @@ auto with_flag(bool on, F f) {
 // because the next row's registers then fit beside the sums; the forward pass, which has no sums, does not care (47.2,
 // 50.3, 53.0).  Backward rows of more than one chunk a thread keep dw's sums in LDS; where registers still run out, the
 // split kernels take them, which read x and dy twice: 4,000 x 24,000 bfloat16 take 186 us with 1,024 x 3 and 262 split,
-// but 312 and 263 with dropout; 2,500 x 32,000 300 and 226; 1,500 x 12,000 double 299 and 165.
+// but 312 and 264 with dropout; 2,500 x 32,000 300 and 227; 1,500 x 12,000 double 299 and 171.
 template <int N> using int_c = std::integral_constant<int, N>;
 template <class T, bool FORWARD, bool DROP, class F>
 bool with_row_shape(int64_t cols, F f) {

@@ -7,7 +7,9 @@ libepi.so (epi_dropout, epi_layer_norm_forward, epi_layer_norm_backward of inclu
 is refused.  Work is enqueued on torch's current stream of the tensor's device, and every array, the workspaces among
 them, is one of torch's, so calls can be captured into a graph (a number as dropout offset is captured with it: every
 replay then drops the same units; a tensor's value is read by every replay).  Leading dimensions are rows, the last
-one the columns; tensors whose rows are evenly spaced are read where they are, others are copied first.
+one the columns; tensors whose rows are evenly spaced over all leading dimensions are read where they are, others (a
+dimension expanded inside of one that moves, columns apart) are copied first.  Derivatives are taken backwards only, and
+once: tensors with a tangent, and second derivatives, are refused.
 """
 import ctypes as C
 

@@ -467,7 +467,8 @@ int32_t epi_layer_norm_forward(const epi_layer_desc *d, const void *x, const voi
 int32_t epi_layer_norm_backward_workspace(const epi_layer_desc *d, size_t *bytes);
 /* dx[rows][cols], dweight[cols] and dbias[cols] (each may be NULL) from x, dy, weight (NULL = ones) and the mean and
  * rstd of the forward pass, with the same dropout, seed and offset.  Sums over the rows are taken in a fixed order in
- * the type of mean and rounded once: the same call gives the same bits.  No output may overlap another array. */
+ * the type of mean and rounded once: the same call gives the same bits.  h - m is taken of the mean as it is stored, so
+ * the gradients of rows with a mean far from zero lose what that rounding takes.  No output may overlap another array. */
 int32_t epi_layer_norm_backward(const epi_layer_desc *d, const void *x, const void *dy, const void *weight,
                                 const void *mean, const void *rstd, void *dx, void *dweight, void *dbias,
                                 void *workspace, size_t workspace_bytes, void *stream);
