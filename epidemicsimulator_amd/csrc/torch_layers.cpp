@@ -524,6 +524,9 @@ PYBIND11_MODULE(_layers, m) {
         take(lib.last_error, a, "epi_last_error");
     });
     // which tensors the calls read where they are, for tests without a GPU
-    m.def("row_distance", [](const Tensor& t) { return row_distance(t.sizes(), t.strides()); });
+    m.def("row_distance", [](const Tensor& t) {
+        if (t.dim() < 1) throw py::value_error("at least one dimension is needed");
+        return row_distance(t.sizes(), t.strides());
+    });
     if (PyModule_AddFunctions(m.ptr(), functions) != 0) throw py::error_already_set();
 }

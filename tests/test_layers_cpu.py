@@ -266,6 +266,12 @@ def test_expanded_dimensions_in_the_middle_are_copied(sizes, strides, want):
     assert layers._layers.row_distance(torch.zeros(4000).as_strided(sizes, strides)) == want
 
 
+def test_rows_of_a_number_are_refused():
+    from epidemicsimulator_amd import layers
+    with pytest.raises(ValueError):
+        layers._layers.row_distance(torch.tensor(1.0))
+
+
 @pytest.mark.parametrize("installed", [True, False])
 def test_build_asks_for_the_binding_where_torch_is_installed(monkeypatch, installed):
     """The library builds without torch, and then nothing loads the binding that was not built."""
