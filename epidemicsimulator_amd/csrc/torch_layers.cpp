@@ -78,6 +78,12 @@ void check_like(const char* name, const Tensor& t, const Tensor& x) {
     if (t.scalar_type() != x.scalar_type()) refuse(std::string(name) + " holds " + str(t.scalar_type()) + ", x holds " + str(x.scalar_type()));
 }
 
+// Fake and zero tensors have shapes and strides, and no memory: a view of one has an address all the same.
+const Tensor& check_memory(const Tensor& t) {
+    if (t.numel() && !t.storage().data()) refuse("a tensor has no memory (a fake tensor, or zeros that were never stored)");
+    return t;
+}
+
 // The distance between rows (the last dimension) that are evenly spaced over all leading dimensions, the last of them
 // running fastest; nothing where they are not, or where a row's columns do not lie next to each other.
 std::optional<int64_t> row_distance(at::IntArrayRef sizes, at::IntArrayRef strides) {
@@ -99,6 +105,7 @@ std::optional<int64_t> row_distance(at::IntArrayRef sizes, at::IntArrayRef strid
 
 // A tensor whose rows are evenly spaced, and their distance: t itself, or a copy.
 std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
+    check_memory(t);
     if (t.is_neg()) return {t.resolve_neg().contiguous(), t.size(-1)};   // a view whose values are the memory's, negated
     if (const auto step = row_distance(t.sizes(), t.strides())) return {t, *step};
     return {t.contiguous(), t.size(-1)};
@@ -108,7 +115,7 @@ Tensor vector_of(const char* name, const Tensor& w, const Tensor& x) {
     if (!w.defined()) return w;
     check_like(name, w, x);
     if (w.dim() != 1 || w.size(0) != x.size(-1)) refuse(std::string(name) + " has the shape " + str(w.sizes()) + " for " + str(x.size(-1)) + " columns");
-    return (w.is_neg() ? w.resolve_neg() : w).contiguous();
+    return (check_memory(w).is_neg() ? w.resolve_neg() : w).contiguous();
 }
 
 // What a call drops with; `offset_dev` may be undefined.
@@ -128,7 +135,7 @@ epi_layer_desc desc_of(const Tensor& x, double eps, const Drop& drop) {
         const Tensor& o = drop.offset_dev;
         if (o.device() != x.device() || o.scalar_type() != at::kLong || o.numel() != 1)
             refuse("offset is a number, or a tensor of one int64 on " + str(x.device()));
-        d.offset_dev = o.data_ptr<int64_t>();
+        d.offset_dev = check_memory(o).data_ptr<int64_t>();
     }
     d.dtype = dtype_of(x);
     d.device = x.get_device();
@@ -470,6 +477,8 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t count
             for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"mean", mean}, {"rstd", rstd}})
                 if (t.device() != x.device() || t.scalar_type() != wide || !t.is_contiguous() || t.is_neg() || t.numel() != rows)
                     refuse(std::string(name) + " is not the forward pass's: " + str(rows) + " numbers of " + str(wide) + " on " + str(x.device()));
+                else
+                    check_memory(t);
             out = run_backward(dy, x, w, mean.data_ptr(), rstd.data_ptr(), drop, true, true, true);
         }
         return triple(out);

@@ -701,3 +701,16 @@ def test_negated_statistics_are_refused(L):
             L.layer_norm_backward(dy, x, w, *args)
         for p, q in zip(L.layer_norm_backward(dy, x, w, *(t.resolve_neg() for t in args)), L.layer_norm_backward(dy, x, w, m, r)):
             assert torch.equal(p, q)
+
+
+def test_zeros_that_were_never_stored_are_refused(L):
+    """Beside tensors that have memory; a stored copy is taken."""
+    from epidemicsimulator_amd import _capi
+    x, w, b, dy = make(4, 8, torch.float32, 82)
+    m, r = L.layer_norm_forward(x, w, b)[1:]
+    plane, line = torch._efficientzerotensor((5, 8), device="cuda")[1:], torch._efficientzerotensor((9,), device="cuda")[1:]
+    for f in (lambda: L.layer_norm(plane, w, b), lambda: L.layer_norm(x, line, b), lambda: L.layer_norm(x, w, line), lambda: L.dropout(plane, 0.5, 1),
+              lambda: L.layer_norm_backward(plane, x, w, m, r), lambda: L.layer_norm_backward(dy, x, w, line[4:], r)):
+        with pytest.raises(_capi.EpiError, match="no memory"):
+            f()
+    assert torch.equal(L.layer_norm(x, w, line.clone()), L.layer_norm(x, w))

@@ -202,6 +202,20 @@ def test_tangents_are_refused():
                 f()
 
 
+def test_tensors_without_memory_are_refused():
+    """Fake tensors of a GPU, whose views have addresses next to zero: refused before anything is enqueued."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from epidemicsimulator_amd import layers
+    with FakeTensorMode():
+        x, w, m = (torch.empty(n, device="cuda:0") for n in ((6, 8), 9, 5))
+        off = torch.empty(2, device="cuda:0", dtype=torch.int64)
+        for f in (lambda: layers.dropout(x, 0.1, 1), lambda: layers.dropout(x[1:], 0.1, 1), lambda: layers.layer_norm(x[1:]), lambda: layers.layer_norm(x[1:], w[1:]),
+                  lambda: layers.layer_norm_forward(x[1:], None, w[1:]), lambda: layers.dropout(x[1:], 0.1, 1, off[1]),
+                  lambda: layers.layer_norm_backward(x[1:], x[:5], None, m, m)):
+            with pytest.raises(_capi.EpiError, match="no memory"):
+                f()
+
+
 def test_two_hip_runtimes_are_refused():
     """libepi.so loaded before torch: the binding says so instead of mixing the two (in a process of its own)."""
     import subprocess
